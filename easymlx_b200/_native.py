@@ -49,6 +49,30 @@ class AttnArgs(C.Structure):
     ]
 
 
+class Visibility(C.Structure):
+    _fields_ = [("tree_mask", C.c_void_p), ("tree_seqs", C.c_void_p), ("tree_words", C.c_int32), ("sink_tokens", C.c_int32)]
+
+
+class Axes(C.Structure):
+    _fields_ = [("positions", C.c_void_p), ("pair_axis", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("axis_stride", C.c_int64), ("num_axes", C.c_int32), ("reserved", C.c_int32)]
+
+
+class StepArgs(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in (
+        "queries", "queries_out", "keys", "values", "query_lens", "slot_ids", "block_tables_all", "kv_lens_all",
+        "query_start_loc", "block_tables", "kv_lens", "ticket", "status", "plan")] + [("plan_bytes", C.c_size_t)] + [
+        (name, C.c_int32) for name in (
+            "in_dtype", "num_seqs", "total_tokens", "num_slots", "max_blocks_per_seq", "advance_kv_lens", "num_q_heads",
+            "sliding_window", "max_query_len", "plan_flags")]
+
+
+class CommitLayer(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in (
+        "key_cache", "value_cache", "k_scale", "k_bias", "v_scale", "v_bias", "block_tables", "kv_lens")] + [
+        ("num_blocks", C.c_int64), ("advance", C.c_int32), ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/easymlx_b200.h
 _I32, _I64, _P = C.c_int32, C.c_int64, C.c_void_p
 SIGNATURES = {
@@ -89,6 +113,15 @@ SIGNATURES = {
     "emlx_copy_blocks": (C.c_int, [C.POINTER(Pool), _P, C.c_int32, _P, C.c_int64, _P, _P]),
     "emlx_zero_pages": (C.c_int, [C.POINTER(Pool), _P, C.c_int32, _P]),
     "emlx_gather_kv_cache": (C.c_int, [C.POINTER(Pool), _P, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32, _P, _P, _P, _P]),
+    "emlx_attn_visible_generic": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Pool), C.POINTER(Visibility), _P]),
+    "emlx_visible_plan_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I32]),
+    "emlx_visible_plan": (C.c_int, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, C.POINTER(Visibility), _I32, _I32, _P, C.c_size_t,
+                                   _P, _P]),
+    "emlx_positioned_step": (C.c_int, [C.POINTER(StepArgs), C.POINTER(Pool), C.POINTER(Rope), C.POINTER(Axes),
+                                      C.POINTER(Visibility), _P]),
+    "emlx_positioned_write": (C.c_int, [_P, _P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _I32, C.POINTER(Rope), C.POINTER(Axes),
+                                       C.POINTER(Visibility), C.POINTER(Pool), _P, _P]),
+    "emlx_commit_tree": (C.c_int, [C.POINTER(CommitLayer), _I32, C.POINTER(Pool), _P, _I32, _P, _I32, _I32, _I32, _P, _P, _P, _P]),
     "emlx_rows_assign": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32, _P]),
     "emlx_rows_update": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32, _P, _P]),
 }
@@ -156,6 +189,22 @@ def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("easymlx_b200 runs on CUDA tensors only; there is no CPU path")
+
+
+class on_device:
+    """Makes a tensor's device current around a launch: a kernel goes to the current device whatever stream it is given."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.before)
 
 
 def launch_count() -> int:

@@ -1,3 +1,3 @@
-from .paged import PageCache, PageCacheConfig, PageCacheView, PageMetadata, build_query_start_loc
+from .paged import PageCache, PageCacheConfig, PageCacheView, PageMetadata, build_query_start_loc, build_tree_mask
 
-__all__ = ("PageCache", "PageCacheConfig", "PageCacheView", "PageMetadata", "build_query_start_loc")
+__all__ = ("PageCache", "PageCacheConfig", "PageCacheView", "PageMetadata", "build_query_start_loc", "build_tree_mask")

@@ -28,6 +28,7 @@ from ... import _native as nv
 
 _CHECK = os.environ.get("EASYMLX_B200_CHECK", "0") not in ("", "0")
 QUANT_GROUP = 64
+MAX_TREE_WORDS = 64  # 64-bit words of a tree mask row
 _FUSED_STEP_MAX_SEQS = 2048  # batch size up to which emlx_kv_write_step serves a batch in one launch
 
 def wide_units_geometry(num_q_heads: int, num_kv_heads: int, head_dim: int) -> bool:
@@ -125,6 +126,14 @@ class PageMetadata:
     # optional host hint from the runner: length of the longest scheduled sequence after this step (0 = unknown);
     # a length-dependent rotary embedding (longrope) picks its table from it without reading the device
     max_kv_len: int = field(default=0, compare=False)
+    # the first tokens of every sequence that stay visible under the sliding window
+    sink_tokens: int = field(default=0, compare=False)
+    # drafted tokens that form a tree: int64 [T, words], bit j of row i = token i sees token j of its sequence (see
+    # build_tree_mask); tree_seqs [S] marks the sequences whose rows follow the mask (None: all), the others are causal
+    tree_mask: tp.Any | None = field(default=None, compare=False)
+    tree_seqs: tp.Any | None = field(default=None, compare=False)
+    # rotary positions of the new tokens, int32 [T] or [axes, T]; None: the token's slot, in a tree its depth
+    rope_positions: tp.Any | None = field(default=None, compare=False)
 
     def with_cache_state(self, *, block_tables, kv_lens, block_size: int) -> "PageMetadata":
         return PageMetadata(
@@ -132,7 +141,8 @@ class PageMetadata:
             block_size=int(block_size), sliding_window=self.sliding_window,
             is_single_token_decode=self.is_single_token_decode, slot_ids=self.slot_ids,
             max_query_len=self.max_query_len, plan=self.plan, query_len_set=self.query_len_set,
-            long_seqs=self.long_seqs,
+            long_seqs=self.long_seqs, sink_tokens=self.sink_tokens, tree_mask=self.tree_mask, tree_seqs=self.tree_seqs,
+            rope_positions=self.rope_positions,
         )
 
     def with_sliding_window(self, sliding_window: int | None) -> "PageMetadata":
@@ -141,7 +151,81 @@ class PageMetadata:
             block_size=self.block_size, sliding_window=sliding_window,
             is_single_token_decode=self.is_single_token_decode, slot_ids=self.slot_ids,
             max_query_len=self.max_query_len, query_len_set=self.query_len_set, long_seqs=self.long_seqs,
+            sink_tokens=self.sink_tokens, tree_mask=self.tree_mask, tree_seqs=self.tree_seqs,
+            rope_positions=self.rope_positions,
         )
+
+
+def build_tree_mask(parents: tp.Sequence[tp.Sequence[int]], device=None) -> torch.Tensor:
+    """Ancestor masks of the trees of one packed batch: ``parents[s][i]`` is the index (inside sequence ``s``'s new tokens)
+    of token ``i``'s parent, ``-1`` for a token that follows the context.  Parents come before their children.  Returns
+    int64 ``[T, words]`` for ``PageMetadata.tree_mask``, ``words = ceil(longest tree / 64)``; every token sees itself, its
+    ancestors and the context."""
+    longest = max((len(p) for p in parents), default=0)
+    words = max(1, -(-longest // 64))
+    if words > MAX_TREE_WORDS:
+        raise ValueError(f"a tree holds at most {64 * MAX_TREE_WORDS} tokens, got {longest}")
+    rows: list[int] = []
+    for s, tree in enumerate(parents):
+        seen: list[int] = []
+        for i, parent in enumerate(tree):
+            parent = int(parent)
+            if not -1 <= parent < i:
+                raise ValueError(f"tree {s}: token {i} has parent {parent}; parents come before their children (-1: the context)")
+            seen.append((seen[parent] if parent >= 0 else 0) | (1 << i))
+        rows.extend(seen)
+    flat = [(row >> (64 * w)) & (2 ** 64 - 1) for row in rows for w in range(words)]
+    mask = torch.tensor([x - 2 ** 64 if x >= 2 ** 63 else x for x in flat], dtype=torch.int64).reshape(len(rows), words)
+    if device is not None and torch.device(device).type == "cuda":
+        return mask.pin_memory().to(device, non_blocking=True)
+    return mask if device is None else mask.to(device)
+
+
+def tree_arguments(tree_mask, tree_seqs, total_tokens: int, num_seqs: int, device) -> tuple[tp.Any, tp.Any]:
+    """``(mask, seqs)`` as the kernels take them: contiguous int64 ``[T, words]`` and int32 ``[S]`` on ``device``."""
+    if tree_mask is None:
+        if tree_seqs is not None:
+            raise ValueError("tree_seqs needs a tree_mask")
+        return None, None
+    if not isinstance(tree_mask, torch.Tensor) or tree_mask.dtype not in (torch.int64, torch.uint64) or tree_mask.ndim != 2:
+        raise ValueError("tree_mask must be an int64 tensor [num_tokens, words] (see build_tree_mask)")
+    if tree_mask.shape[0] != total_tokens or not 1 <= tree_mask.shape[1] <= MAX_TREE_WORDS:
+        raise ValueError(f"tree_mask must be [{total_tokens}, 1..{MAX_TREE_WORDS}], got {tuple(tree_mask.shape)}")
+    if tree_mask.device != device:
+        raise ValueError("tree_mask must be on the device of the queries")
+    if tree_seqs is not None:
+        if not isinstance(tree_seqs, torch.Tensor):
+            tree_seqs = torch.as_tensor(tree_seqs)
+        if tree_seqs.ndim != 1 or tree_seqs.shape[0] != num_seqs or tree_seqs.dtype.is_floating_point:
+            raise ValueError(f"tree_seqs must be [{num_seqs}] integers or truth values")
+        if tree_seqs.is_cuda and tree_seqs.device != device:
+            raise ValueError("tree_seqs must be on the device of the queries")
+        if tree_seqs.dtype != torch.int32 or tree_seqs.device != device:
+            tree_seqs = (tree_seqs != 0).to(device=device, dtype=torch.int32)
+        tree_seqs = tree_seqs.contiguous()
+    return tree_mask.contiguous(), tree_seqs
+
+
+def native_visibility(sink_tokens: int, tree_mask, tree_seqs) -> nv.Visibility:
+    v = nv.Visibility()
+    v.sink_tokens = int(sink_tokens)
+    if tree_mask is not None:
+        v.tree_mask, v.tree_words = tree_mask.data_ptr(), int(tree_mask.shape[1])
+        if tree_seqs is not None:
+            v.tree_seqs = tree_seqs.data_ptr()
+    return v
+
+
+class VisiblePlan(tp.NamedTuple):
+    """Work list of a step with sinks or a tree, and what it was built for."""
+
+    buffer: torch.Tensor
+    num_q_heads: int
+    sliding_window: int
+    flags: int
+    sink_tokens: int
+    tree_mask: tp.Any
+    tree_seqs: tp.Any
 
 
 def expanded_page_hint(query_lens, group: int) -> int:
@@ -313,6 +397,15 @@ class PageCacheView:
             raise IndexError(f"Invalid seq_idx {seq_idx}")
         return int(self.kv_lens[seq_idx].item()) + int(num_new_tokens) <= self.max_seq_len
 
+    def _commit_geometry(self) -> tuple:
+        for t in (self.block_tables, self.kv_lens):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError("block_tables and kv_lens must be contiguous int32")
+        if not (self.key_cache.is_contiguous() and self.value_cache.is_contiguous()):
+            raise ValueError("key_cache and value_cache must be contiguous")
+        return (self.block_size, self.num_kv_heads, self.head_dim, self.cache_bits, self.key_cache.dtype, self.num_seqs,
+                self.blocks_per_seq, self.key_cache.device)
+
     # ------------------------------------------------------------------ native descriptors
     def native_pool(self) -> nv.Pool:
         p = nv.Pool()
@@ -408,6 +501,94 @@ class PageCacheView:
         if _CHECK and not torch.cuda.is_current_stream_capturing():
             self.check()
         return qsl, bt, lens, (None if plan is None else (plan, hq, window, flags)), rotated_q
+
+    def _write_positioned(self, keys, values, query_lens_dev, slots_dev, total: int, queries, *, rope, positions, window: int,
+                          max_q: int, long_seqs: int, advance: bool, sinks: int, tree_mask, tree_seqs):
+        """``_write_batch`` for a step with sinks, a draft tree or given rotary positions (``query_lens_dev`` ``None``: one
+        token per sequence): the rows, the metadata and the work list of ``visible_attention`` in one launch."""
+        nv.require_cuda(keys, values, queries, self.key_cache)
+        dev, lib = self.key_cache.device, nv.lib()
+        if self.block_tables.dtype != torch.int32 or self.kv_lens.dtype != torch.int32:
+            raise ValueError("block_tables and kv_lens must be int32")
+        if not (self.block_tables.is_contiguous() and self.kv_lens.is_contiguous()):
+            raise ValueError("block_tables and kv_lens must be contiguous")
+        s = int(slots_dev.shape[0])
+        if total > 0:
+            if keys.shape != values.shape:
+                raise ValueError("key and value must have the same shape")
+            if keys.ndim != 3 or tuple(keys.shape) != (total, self.num_kv_heads, self.head_dim):
+                raise ValueError("key/value must be [num_tokens, num_kv_heads, head_dim] matching the cache")
+            if queries.ndim != 3 or queries.shape[0] != total:
+                raise ValueError("queries must be rank-3: [total_tokens, num_q_heads, head_dim]")
+            if keys.dtype != values.dtype:
+                raise ValueError("key and value must have the same dtype")
+            if any(t.device != dev for t in (keys, values, queries)):
+                raise ValueError("queries, keys and values must be on the device of the cache")
+            keys, values = keys.contiguous(), values.contiguous()
+        hq = int(queries.shape[1])
+        qsl = torch.empty(s + 1, dtype=torch.int32, device=dev) if s else torch.zeros(1, dtype=torch.int32, device=dev)
+        bt = torch.empty((s, self.blocks_per_seq), dtype=torch.int32, device=dev)
+        lens = torch.empty(s, dtype=torch.int32, device=dev)
+        native_rope = axes = rotated_q = None
+        if rope is not None and total > 0:
+            if not hasattr(rope, "native_axes"):
+                raise TypeError("rope must be an easymlx_b200.layers.rotary.RotaryEmbedding (see get_rope)")
+            if queries.dtype != keys.dtype or queries.shape[2] != self.head_dim:
+                raise ValueError("queries and keys must have the same dtype and head_dim when RoPE is fused into the write")
+            if positions is not None:
+                positions = rope.checked_positions(positions, total, dev)
+            native_rope, axes = rope.native(dev), rope.native_axes(dev, positions)
+            queries = queries.contiguous()
+            rotated_q = torch.empty_like(queries)
+        vis = native_visibility(sinks, tree_mask, tree_seqs)
+        words = 0 if tree_mask is None else int(tree_mask.shape[1])
+        plan, plan_bytes, flags = None, 0, 0
+        visible = tree_mask is not None or (sinks > 0 and window > 0)
+        if visible and total > 0 and hq % self.num_kv_heads == 0 and (
+                self.block_size == 128 or (not self.is_affine and self.block_size in (16, 32, 64))):
+            flags = visible_plan_flags(self.cache_bits if self.is_affine else 0, hq, self.num_kv_heads, self.head_dim, long_seqs)
+            plan_bytes = int(lib.emlx_visible_plan_bytes(s, total, hq, self.num_kv_heads, words))
+            plan = torch.empty(plan_bytes, dtype=torch.uint8, device=dev)
+        with nv.on_device(dev):
+            stream = nv.stream_ptr(dev)
+            if s <= _FUSED_STEP_MAX_SEQS:
+                a = nv.StepArgs()
+                if rotated_q is not None:
+                    a.queries, a.queries_out = queries.data_ptr(), rotated_q.data_ptr()
+                a.keys, a.values = keys.data_ptr(), values.data_ptr()
+                a.query_lens = None if query_lens_dev is None else query_lens_dev.data_ptr()
+                a.slot_ids, a.block_tables_all, a.kv_lens_all = slots_dev.data_ptr(), self.block_tables.data_ptr(), self.kv_lens.data_ptr()
+                a.query_start_loc, a.block_tables, a.kv_lens = qsl.data_ptr(), bt.data_ptr(), lens.data_ptr()
+                a.ticket, a.status = self.ticket.data_ptr(), self.status.data_ptr()
+                if plan is not None:
+                    a.plan, a.plan_bytes = plan.data_ptr(), plan_bytes
+                a.in_dtype, a.num_seqs, a.total_tokens, a.num_slots = nv.dtype_code(keys.dtype), s, total, self.num_seqs
+                a.max_blocks_per_seq, a.advance_kv_lens, a.num_q_heads = self.blocks_per_seq, int(bool(advance)), hq
+                a.sliding_window, a.max_query_len, a.plan_flags = window, max_q, flags
+                nv.check(lib.emlx_positioned_step(a, self.native_pool(), native_rope, axes, vis, stream))
+            else:
+                ones = query_lens_dev if query_lens_dev is not None else torch.ones(s, dtype=torch.int32, device=dev)
+                slot_mapping = torch.empty(max(total, 1), dtype=torch.int64, device=dev)
+                token_positions = torch.empty(max(total, 1), dtype=torch.int32, device=dev)
+                nv.check(lib.emlx_build_metadata(
+                    nv.ptr(ones), nv.ptr(slots_dev), s, total, nv.ptr(self.block_tables), self.num_seqs, self.blocks_per_seq,
+                    nv.ptr(self.kv_lens), self.block_size, 1 if advance else 0, nv.ptr(qsl), nv.ptr(bt), nv.ptr(lens),
+                    nv.ptr(slot_mapping), nv.ptr(token_positions), self.num_blocks, nv.ptr(self.status), 0, 0, 0, 0, 0, None, 0,
+                    stream))
+                nv.check(lib.emlx_positioned_write(
+                    nv.ptr(queries) if rotated_q is not None else None, nv.ptr(rotated_q), hq, nv.ptr(keys), nv.ptr(values),
+                    nv.dtype_code(keys.dtype), total, nv.ptr(slot_mapping), nv.ptr(token_positions), nv.ptr(qsl), s, native_rope,
+                    axes, vis, self.native_pool(), nv.ptr(self.status), stream))
+                plan = None  # built by the attention call
+        if _CHECK and not torch.cuda.is_current_stream_capturing():
+            self.check()
+        return (qsl, bt, lens, None if plan is None else VisiblePlan(plan, hq, window, flags, sinks, tree_mask, tree_seqs),
+                rotated_q, positions)
+
+    # ------------------------------------------------------------------ draft trees
+    def commit_tree(self, slot_ids, accepted, *, advance: bool = True) -> torch.Tensor:
+        """Keep the accepted path of every scheduled sequence's tree and drop the rest; see ``PageCache.commit_tree``."""
+        return commit_layers([self], slot_ids, accepted, advance=advance)
 
     def append(self, seq_idx: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Append ``[num_tokens, num_kv_heads, head_dim]`` rows to one slot (``cache.py:834-872``)."""
@@ -584,6 +765,31 @@ class PageCacheView:
             rope = rope.select(longest)
         group = max(1, int(queries.shape[1]) // self.num_kv_heads)
         long_seqs = expanded_page_hint(qlens, group)
+        sinks = int(getattr(cache_metadata, "sink_tokens", 0) or 0)
+        tree_mask, tree_seqs = getattr(cache_metadata, "tree_mask", None), getattr(cache_metadata, "tree_seqs", None)
+        positions = getattr(cache_metadata, "rope_positions", None)
+        if sinks < 0:
+            raise ValueError("sink_tokens must be non-negative")
+        if tree_mask is not None or tree_seqs is not None or positions is not None or (sinks and window > 0):
+            tree_mask, tree_seqs = tree_arguments(tree_mask, tree_seqs, total, len(slots), dev)
+            if tree_mask is not None and qlens and tree_seqs is None and max_q > 64 * tree_mask.shape[1]:
+                raise ValueError(f"a tree of {max_q} tokens needs {-(-max_q // 64)} mask words, got {tree_mask.shape[1]}")
+            if positions is not None and rope is None:
+                raise ValueError("rope_positions needs a rope")
+            qsl, bt, lens, plan, rotated_q, keep = self._write_positioned(
+                keys, values, None if single and len(slots) == total else qlens_dev, _uploaded.get(slots, dev), total,
+                queries, rope=rope, positions=positions, window=window, max_q=max_q, long_seqs=long_seqs, advance=advance,
+                sinks=sinks, tree_mask=tree_mask, tree_seqs=tree_seqs)
+            if rotated_q is not None:
+                queries = rotated_q
+            meta = PageMetadata(
+                query_start_loc=qsl, sliding_window=getattr(cache_metadata, "sliding_window", None),
+                is_single_token_decode=bool(getattr(cache_metadata, "is_single_token_decode", False)) or single,
+                slot_ids=getattr(cache_metadata, "slot_ids", None) or slots, max_query_len=max_q, plan=plan,
+                query_len_set=None if qlens is None else tuple(sorted(set(q for q in qlens if q > 0))),
+                long_seqs=long_seqs, sink_tokens=sinks, tree_mask=tree_mask, tree_seqs=tree_seqs, rope_positions=keep,
+            ).with_cache_state(block_tables=bt, kv_lens=lens, block_size=self.block_size)
+            return queries, self.key_cache, self.value_cache, meta
         qsl, bt, lens, plan, rotated_q = self._write_batch(
             keys, values, qlens_dev, _uploaded.get(slots, dev), total,
             plan_for=(int(queries.shape[1]), window, max_q, long_seqs), advance=advance, rope=rope, queries=queries,
@@ -598,6 +804,67 @@ class PageCacheView:
             long_seqs=long_seqs,
         ).with_cache_state(block_tables=bt, kv_lens=lens, block_size=self.block_size)
         return queries, self.key_cache, self.value_cache, meta
+
+
+def visible_plan_flags(bits: int, num_q_heads: int, num_kv_heads: int, head_dim: int, long_seqs: int) -> int:
+    """Flags of a ``VisiblePlan``: over an affine pool, rows beyond 16 go to the tcgen05 kernel when their pages are expanded
+    for it (``long_seqs``)."""
+    flags = int(nv.lib().emlx_attn_plan_flags(bits, num_q_heads, num_kv_heads, head_dim))
+    if bits and long_seqs > 0 and wide_units_geometry(num_q_heads, num_kv_heads, head_dim):
+        flags |= 1
+    return flags
+
+
+def commit_layers(views: tp.Sequence[PageCacheView], slot_ids, accepted, *, advance: bool = True) -> torch.Tensor:
+    """The launch behind every ``commit_tree``: the views are the layers of one cache, alike in geometry and format."""
+    if not views:
+        raise ValueError("commit_tree needs at least one layer")
+    first = views[0]
+    dev, geometry = first.key_cache.device, first._commit_geometry()
+    layers = (nv.CommitLayer * len(views))()
+    for layer, view in zip(layers, views):
+        if view is not first and view._commit_geometry() != geometry:
+            raise ValueError("commit_tree needs layers of the same geometry, format and device")
+        layer.key_cache, layer.value_cache = view.key_cache.data_ptr(), view.value_cache.data_ptr()
+        if view.is_affine:
+            layer.k_scale, layer.k_bias = view.k_scales.data_ptr(), view.k_biases.data_ptr()
+            layer.v_scale, layer.v_bias = view.v_scales.data_ptr(), view.v_biases.data_ptr()
+        layer.block_tables, layer.kv_lens = view.block_tables.data_ptr(), view.kv_lens.data_ptr()
+        layer.num_blocks, layer.advance = view.num_blocks, int(bool(advance))
+    nv.require_cuda(first.key_cache)
+    if isinstance(slot_ids, torch.Tensor):
+        if slot_ids.ndim != 1 or slot_ids.dtype.is_floating_point:
+            raise ValueError("slot_ids must be rank-1 integers")
+        slots = slot_ids.to(device=dev, dtype=torch.int32).contiguous()
+    else:
+        host = tuple(int(x) for x in slot_ids)
+        if len(set(host)) != len(host):
+            raise ValueError("a slot id must not appear twice in one batch")
+        if any(x < 0 or x >= first.num_seqs for x in host):
+            raise IndexError(f"Invalid slot id in {host}")
+        slots = _uploaded.get(host, dev)
+    s = int(slots.shape[0])
+    if not isinstance(accepted, torch.Tensor):
+        rows = [[int(x) for x in row] for row in accepted]
+        width = max((len(row) for row in rows), default=0)
+        if any(b <= a for row in rows for a, b in zip([-1] + row[:-1], row)):
+            raise ValueError("an accepted path lists token indices in increasing order")
+        accepted = torch.tensor([row + [-1] * (width - len(row)) for row in rows], dtype=torch.int32).reshape(len(rows), width)
+    if accepted.ndim != 2 or accepted.shape[0] != s or accepted.dtype.is_floating_point:
+        raise ValueError(f"accepted must be integers [{s}, max_path], ended by -1")
+    if accepted.is_cuda and accepted.device != dev:
+        raise ValueError("accepted must be on the device of the cache")
+    accepted = accepted.to(device=dev, dtype=torch.int32).contiguous()
+    committed = torch.empty(s, dtype=torch.int32, device=dev)
+    if s == 0:
+        return committed
+    with nv.on_device(dev):
+        nv.check(nv.lib().emlx_commit_tree(layers, len(views), first.native_pool(), nv.ptr(slots), s, nv.ptr(accepted),
+                                           int(accepted.shape[1]), first.num_seqs, first.blocks_per_seq, nv.ptr(committed),
+                                           nv.ptr(first.ticket), nv.ptr(first.status), nv.stream_ptr(dev)))
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
+        first.check()
+    return committed
 
 
 class PageCacheConfig:
@@ -656,10 +923,21 @@ class PageCache:
         for view in self.views:
             view.clear()
 
+    def commit_tree(self, slot_ids, accepted, *, advance: bool = True) -> torch.Tensor:
+        """Keep the accepted path of every scheduled sequence's draft tree, in all layers.
+
+        The trees were written behind the context with ``concatenate_to_cache(..., advance=False)``, so ``kv_lens`` still
+        holds the context lengths.  ``accepted`` ``[num_seqs, max_path]`` lists, per entry of ``slot_ids``, the indices of
+        the accepted new tokens in increasing order, ended by ``-1`` (a device tensor, or host lists of any lengths).
+        Token ``accepted[i, j]``'s rows move to position ``context + j`` and (unless ``advance=False``) the stored length
+        becomes the context plus the path.  Returns the lengths after the step, int32 ``[num_seqs]``.  One launch for up
+        to 32 layers.  A device-side path that is not increasing leaves its sequence alone and is reported by ``check``."""
+        return commit_layers(self.views, slot_ids, accepted, advance=advance)
+
     def copy_blocks(self, block_mapping) -> None:
         """Copy pages in every layer's pool (``caching/paged/cache.py:1437-1445``)."""
         for view in self.views:
             view.copy_blocks(block_mapping)
 
 
-__all__ = ("PageCache", "PageCacheConfig", "PageCacheView", "PageMetadata", "build_query_start_loc")
+__all__ = ("PageCache", "PageCacheConfig", "PageCacheView", "PageMetadata", "build_query_start_loc", "build_tree_mask")

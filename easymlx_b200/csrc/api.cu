@@ -57,12 +57,13 @@ int emlx_read_status(const int32_t* status, void* stream) {
     EMLX_CUDA_OK(cudaMemcpyAsync(&host, status, sizeof(host), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     EMLX_CUDA_OK(cudaStreamSynchronize((cudaStream_t)stream));
     if (host == 0) return EMLX_OK;
-    return emlx::fail(EMLX_ERR_DEVICE, "device status 0x%x:%s%s%s%s%s", host,
+    return emlx::fail(EMLX_ERR_DEVICE, "device status 0x%x:%s%s%s%s%s%s", host,
                       (host & EMLX_DEV_BAD_SLOT) ? " slot id out of range;" : "",
                       (host & EMLX_DEV_BAD_PAGE) ? " page id out of range inside a live sequence;" : "",
                       (host & EMLX_DEV_OVERFLOW) ? " sequence outgrows its page-table row;" : "",
                       (host & EMLX_DEV_TOKEN_MISMATCH) ? " sum(query_lens) != total_tokens;" : "",
-                      (host & EMLX_DEV_WAIT_TIMEOUT) ? " in-kernel wait timed out;" : "");
+                      (host & EMLX_DEV_WAIT_TIMEOUT) ? " in-kernel wait timed out;" : "",
+                      (host & EMLX_DEV_BAD_TREE) ? " tree mask too narrow or accepted path not increasing;" : "");
 }
 
 }  // extern "C"

@@ -61,11 +61,12 @@ __device__ __forceinline__ void unit_tiles(int row0, int row1, int G, int q_len,
 // cost, kTileCost per tile + part_cost(c) per (unit, head) part (measured on the 8-row decode kernel: a part
 // boundary costs about as much as 2.3 tiles).  `cum` is the exclusive prefix sum of tiles per unit (num_units + 1).
 // Only the first `used` CTAs receive work (the others get empty slices and leave at once).
+template <int THREADS = kMetaThreads>
 __device__ __forceinline__ void cut_slices(int c, const int32_t* cum, int num_units, int tile_base, int Hkv,
                                            int num_ctas, int32_t* plan, const PlanLayout& L, int used) {
     const int tid = threadIdx.x;
     {
-        for (int i = tid; i <= num_ctas; i += kMetaThreads) {
+        for (int i = tid; i <= num_ctas; i += THREADS) {
             long long start = (long long)tile_base * Hkv;
             int first_unit = num_units;
             const long long kPartCost = part_cost(c);

@@ -22,7 +22,7 @@ import torch
 
 from ...._native import EMLX_OK  # noqa: F401  (re-exported for callers that test return codes)
 from .... import _native as nv
-from ....caching.paged.cache import PageCacheView, PageMetadata, _uploaded, build_query_start_loc
+from ....caching.paged.cache import PageCacheView, PageMetadata, _uploaded, build_query_start_loc, commit_layers
 from .execution_types import ScheduledSequence, build_positions
 
 
@@ -109,6 +109,10 @@ class PageTableRunner:
             return
         for cache in self.kv_caches:
             cache.zero_pages(valid)
+
+    def commit_tree(self, slot_ids, accepted, *, advance: bool = True) -> torch.Tensor:
+        """Keep the accepted path of every scheduled sequence's draft tree in every cache (``PageCache.commit_tree``)."""
+        return commit_layers(self.kv_caches, slot_ids, accepted, advance=advance)
 
     # ------------------------------------------------------------------ batch format
     @staticmethod

@@ -1,3 +1,3 @@
-from .rotary import LongRopeEmbedding, RotaryEmbedding, get_rope
+from .rotary import LongRopeEmbedding, MultiAxisRotaryEmbedding, RotaryEmbedding, get_rope
 
-__all__ = ("LongRopeEmbedding", "RotaryEmbedding", "get_rope")
+__all__ = ("LongRopeEmbedding", "MultiAxisRotaryEmbedding", "RotaryEmbedding", "get_rope")

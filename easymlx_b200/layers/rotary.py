@@ -47,6 +47,58 @@ class RotaryEmbedding:
         r.head_dim_if_no_pool = int(head_dim)
         return r
 
+    # ------------------------------------------------------------------ positions given per token (and axis)
+    num_axes = 1
+
+    def pair_axis(self, device) -> torch.Tensor | None:
+        """Axis of every pair as uint8 ``[dims / 2]``; ``None``: one axis."""
+        return None
+
+    def inv_freq64(self, device) -> torch.Tensor:
+        """Radians per position of every pair, the position scale included: the angle of a far position is a product that
+        32 bits cannot hold to the accuracy of the rotation, so its factors are kept in 64."""
+        key = "f64:" + str(device)
+        if key not in self._inv_freq:
+            self._inv_freq[key] = torch.from_numpy(self.scale / self.freqs.astype(np.float64)).to(device)
+        return self._inv_freq[key]
+
+    def checked_positions(self, positions, tokens: int, device) -> torch.Tensor:
+        """``positions`` as contiguous int32 ``[axes, tokens]`` on the device: ``[tokens]`` or ``[1, tokens]`` (the same on
+        every axis) or one row per axis."""
+        pos = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(positions)
+        if pos.dtype.is_floating_point or pos.dtype.is_complex or pos.dtype == torch.bool:
+            raise ValueError("rope positions must be integers")
+        if pos.ndim == 1:
+            pos = pos[None]
+        if pos.ndim != 2 or pos.shape[1] != tokens or pos.shape[0] not in (1, self.num_axes):
+            raise ValueError(f"rope positions must be [num_tokens] or [{self.num_axes}, num_tokens] with num_tokens = {tokens}, "
+                             f"got {tuple(positions.shape) if isinstance(positions, torch.Tensor) else tuple(pos.shape)}")
+        if isinstance(positions, torch.Tensor) and positions.is_cuda and positions.device != device:
+            raise ValueError("rope positions must be on the device of the rows")
+        return pos.to(device=device, dtype=torch.int32).contiguous()
+
+    def native_axes(self, device, positions: torch.Tensor | None) -> nv.Axes:
+        """``positions`` as ``checked_positions`` returns them; ``None``: the kernel's own (slot, or depth in a tree)."""
+        a = nv.Axes()
+        a.inv_freq = self.inv_freq64(device).data_ptr()
+        if positions is not None:
+            a.positions, a.num_axes, a.axis_stride = positions.data_ptr(), int(positions.shape[0]), int(positions.shape[1])
+            if positions.shape[0] > 1:
+                a.pair_axis = self.pair_axis(device).data_ptr()
+        return a
+
+    def _apply_axes(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        out = torch.empty_like(x)
+        t, h, d = x.shape
+        if t == 0:
+            return out
+        rope = self.native(x.device, head_dim=d)
+        with nv.on_device(x.device):
+            nv.check(nv.lib().emlx_positioned_write(
+                nv.ptr(x), nv.ptr(out), h, None, None, nv.dtype_code(x.dtype), t, None, None, None, 0, rope,
+                self.native_axes(x.device, positions), None, None, None, nv.stream_ptr(x.device)))
+        return out
+
     def __call__(self, x: torch.Tensor, offset: int | torch.Tensor = 0) -> torch.Tensor:
         """Rotate ``x`` (``[B, H, L, D]`` with positions ``offset + arange(L)``, or ``[T, H, D]`` with ``offset`` a
         tensor of T positions)."""
@@ -74,6 +126,51 @@ class RotaryEmbedding:
         nv.check(nv.lib().emlx_kv_write_rope(nv.ptr(x), nv.ptr(out), h, None, None, nv.dtype_code(x.dtype), t, None,
                                              nv.ptr(positions), rope, None, None, nv.stream_ptr(x.device)))
         return out
+
+
+class MultiAxisRotaryEmbedding(RotaryEmbedding):
+    """Rotary embedding whose pairs are shared out over several position axes (time, height, width of a picture or a video).
+
+    ``sections`` holds the number of pairs of every axis (their sum is ``dims / 2``).  Pairs are dealt in blocks (the first
+    ``sections[0]`` pairs to axis 0, and so on) or, with ``interleaved``, in turn: pair ``i`` belongs to axis ``i % A``
+    while that axis has pairs left (``i < A * sections[axis]``), else to axis 0.
+
+    Positions come as ``[axes, T]``: through ``PageMetadata.rope_positions`` for a step of the cache, as ``offset`` for a
+    tensor on its own (``rope(x, offset=positions)`` with ``x`` ``[T, H, D]``).  Without them it rotates like the plain
+    embedding (text: all axes agree).
+    """
+
+    def __init__(self, dims: int, base: float = 10000.0, traditional: bool = False, scale: float = 1.0, freqs=None,
+                 mscale: float = 1.0, *, sections: tp.Sequence[int], interleaved: bool = False):
+        super().__init__(dims, base=base, traditional=traditional, scale=scale, freqs=freqs, mscale=mscale)
+        self.sections, self.interleaved = tuple(int(x) for x in sections), bool(interleaved)
+        if not self.sections or min(self.sections) < 0 or sum(self.sections) != self.dims // 2 or len(self.sections) > 255:
+            raise ValueError(f"sections must be non-negative and add up to dims / 2 = {self.dims // 2}, got {self.sections}")
+        self.num_axes = len(self.sections)
+        pair = np.arange(self.dims // 2)
+        if self.interleaved:
+            axis = pair % self.num_axes
+            owned = np.where((axis > 0) & (pair < self.num_axes * np.asarray(self.sections)[axis]), axis, 0)
+            if any((owned == a).sum() != n for a, n in enumerate(self.sections)):
+                raise ValueError(f"sections {self.sections} cannot be interleaved over {self.dims // 2} pairs")
+            self._axis_of_pair = owned.astype(np.uint8)
+        else:
+            self._axis_of_pair = np.repeat(np.arange(self.num_axes), self.sections).astype(np.uint8)
+        self._pair_axis: dict[str, torch.Tensor] = {}
+
+    def pair_axis(self, device) -> torch.Tensor:
+        key = str(device)
+        if key not in self._pair_axis:
+            self._pair_axis[key] = torch.from_numpy(self._axis_of_pair).to(device)
+        return self._pair_axis[key]
+
+    def __call__(self, x: torch.Tensor, offset: int | torch.Tensor = 0) -> torch.Tensor:
+        if not (torch.is_tensor(offset) and offset.ndim == 2):
+            return super().__call__(x, offset=offset)
+        nv.require_cuda(x)
+        if x.ndim != 3:
+            raise ValueError("with positions per axis, x must be [T, H, D]")
+        return self._apply_axes(x.contiguous(), self.checked_positions(offset, int(x.shape[0]), x.device))
 
 
 class LongRopeEmbedding:
@@ -147,6 +244,10 @@ def get_rope(dims: int, base: float, traditional: bool, scaling_config: dict | N
     kind = "default"
     if scaling_config is not None:
         kind = scaling_config.get("type") or scaling_config.get("rope_type", "default")
+    sections = (scaling_config or {}).get("mrope_section")
+    if kind == "mrope" and sections is not None and sum(sections) == int(dims) // 2:
+        return MultiAxisRotaryEmbedding(int(dims), base=base, traditional=traditional, sections=sections,
+                                        interleaved=bool(scaling_config.get("mrope_interleaved", False)))
     if kind in ("default", "linear", "mrope"):
         scale = 1 / scaling_config["factor"] if kind == "linear" else 1.0
         return RotaryEmbedding(int(dims), base=base, traditional=traditional, scale=scale)
@@ -166,4 +267,4 @@ def get_rope(dims: int, base: float, traditional: bool, scaling_config: dict | N
     raise ValueError(f"Unsupported RoPE type {kind}")
 
 
-__all__ = ("LongRopeEmbedding", "RotaryEmbedding", "get_rope")
+__all__ = ("LongRopeEmbedding", "MultiAxisRotaryEmbedding", "RotaryEmbedding", "get_rope")

@@ -320,6 +320,9 @@ def paged_attention(
     query_len_set: tp.Sequence[int] | None = None,
     gather=None,
     long_seqs: int = 0,
+    sink_tokens: int = 0,
+    tree_mask: torch.Tensor | None = None,
+    tree_seqs=None,
 ) -> torch.Tensor:
     """Ragged causal attention of packed queries over a paged KV pool.
 
@@ -333,10 +336,29 @@ def paged_attention(
     an entry point explicitly; tests and benchmarks use it.  ``long_seqs`` (the number of sequences with more than 16
     query rows, another host hint) lets an affine pool serve those rows on the tcgen05 kernel.  ``gather`` (a ``distributed.GatherTarget``) makes the call
     store its heads into every rank's full output (KV heads sharded over GPUs) and return this rank's copy of it.
+
+    ``sink_tokens`` first tokens of every sequence stay visible under the sliding window (without a window they change
+    nothing).  ``tree_mask`` (int64 ``[T, words]``, see ``build_tree_mask``) makes the new tokens of a sequence a tree of
+    drafts: bit ``j`` of a token's mask says whether it sees the sequence's new token ``j``; the context stays visible.
+    ``tree_seqs`` (``[S]``) names the sequences the mask is for when others of the batch are causal.
     """
     del use_metal, threadgroup_size, allow_fallback
     if single_token_decode and not max_query_len:
         max_query_len = 1
+    if int(sink_tokens or 0) < 0:
+        raise ValueError("sink_tokens must be non-negative")
+    if tree_mask is not None or tree_seqs is not None or (sink_tokens and sliding_window):
+        from .visible_attention import VisibleAttentionCall
+
+        if gather is not None:
+            raise NotImplementedError("a gathering call takes neither sinks nor a tree")
+        return VisibleAttentionCall(queries, key_cache, value_cache, block_tables, kv_lens, query_start_loc,
+                                    softmax_scale=softmax_scale, sliding_window=sliding_window, sink_tokens=sink_tokens,
+                                    tree_mask=tree_mask, tree_seqs=tree_seqs, k_scale=k_scale, v_scale=v_scale, k_bias=k_bias,
+                                    v_bias=v_bias, kernel=kernel, max_query_len=max_query_len, plan=plan,
+                                    query_len_set=query_len_set, long_seqs=long_seqs).plan().launch()
+    if plan is not None and len(plan) != 4:
+        plan = None  # the work list of a call with sinks or a tree
     return AttentionCall(queries, key_cache, value_cache, block_tables, kv_lens, query_start_loc,
                          softmax_scale=softmax_scale, sliding_window=sliding_window, k_scale=k_scale, v_scale=v_scale,
                          k_bias=k_bias, v_bias=v_bias, kernel=kernel, max_query_len=max_query_len,
@@ -393,7 +415,9 @@ class UnifiedAttention(BaseOperation):
             single_token_decode=cache_metadata.is_single_token_decode,
             max_query_len=int(getattr(cache_metadata, "max_query_len", 0) or 0),
             plan=getattr(cache_metadata, "plan", None), query_len_set=getattr(cache_metadata, "query_len_set", None),
-            long_seqs=int(getattr(cache_metadata, "long_seqs", 0) or 0), **extra,
+            long_seqs=int(getattr(cache_metadata, "long_seqs", 0) or 0),
+            sink_tokens=int(getattr(cache_metadata, "sink_tokens", 0) or 0),
+            tree_mask=getattr(cache_metadata, "tree_mask", None), tree_seqs=getattr(cache_metadata, "tree_seqs", None), **extra,
         )
         return AttentionOutput(attention_outputs=outputs, cache_view=cache_view)
 

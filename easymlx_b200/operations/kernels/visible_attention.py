@@ -1,0 +1,108 @@
+"""Paged attention of rows that see something else than a causal window: sliding windows whose first tokens stay
+visible, and trees of drafted tokens.  ``paged_attention(sink_tokens=..., tree_mask=...)`` comes here.
+
+A row's *visible sequence* is the context followed by the new tokens its mask names, in slot order (a causal row: those
+up to itself).  A sliding window keeps its last ``sliding_window`` entries and ``sink_tokens`` its first ones; a row
+that sees nothing gets zeros.
+"""
+
+from __future__ import annotations
+
+import math
+import typing as tp
+
+import torch
+
+from ... import _native as nv
+from .unified_attention import (_CHECK, _TILED_BLOCK_SIZE_AFFINE, _TILED_BLOCK_SIZES_FLOAT, _TILED_HEAD_DIMS, _as_int32,
+                                _make_pool, _scratch, _validate_inputs)
+
+
+class VisibleAttentionCall:
+    """One validated call, split like ``AttentionCall`` into ``plan()`` (work list) and ``launch()``.
+
+    Work list and workspace belong to the call (the counters in them are set up by the work list), so calls on different
+    streams and captured graphs share nothing but the status word."""
+
+    def __init__(self, queries, key_cache, value_cache, block_tables, kv_lens, query_start_loc, *,
+                 softmax_scale: float | None = None, sliding_window: int | None = None, sink_tokens: int = 0, tree_mask=None,
+                 tree_seqs=None, k_scale=None, v_scale=None, k_bias=None, v_bias=None, kernel: str | None = None,
+                 max_query_len: int = 0, plan=None, query_len_set: tp.Sequence[int] | None = None, long_seqs: int = 0):
+        from ...caching.paged.cache import VisiblePlan, native_visibility, tree_arguments, visible_plan_flags
+
+        nv.require_cuda(queries, key_cache, value_cache)
+        dev = queries.device
+        if key_cache.device != dev or value_cache.device != dev:
+            raise ValueError("queries, key_cache and value_cache must be on one device")
+        affine = key_cache.dtype == torch.uint8
+        self.block_tables, self.kv_lens = _as_int32(block_tables, dev), _as_int32(kv_lens, dev)
+        self.query_start_loc = _as_int32(query_start_loc, dev)
+        _validate_inputs(queries, key_cache, value_cache, self.block_tables, self.kv_lens, self.query_start_loc, affine)
+        if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("key_cache and value_cache must be contiguous")
+        if kernel not in (None, "generic", "tiled"):
+            raise ValueError("a call with sinks or a tree takes kernel=None, 'generic' or 'tiled'")
+        if int(sink_tokens) < 0 or int(sliding_window or 0) < 0:
+            raise ValueError("sink_tokens and sliding_window must be non-negative")
+        self.device = dev
+        self.total, self.hq, self.d = (int(x) for x in queries.shape)
+        self.num_seqs = int(self.block_tables.shape[0])
+        if self.kv_lens.shape[0] != self.num_seqs:
+            raise ValueError("kv_lens must have length num_seqs")
+        self.tree_mask, self.tree_seqs = tree_arguments(tree_mask, tree_seqs, self.total, self.num_seqs, dev)
+        if self.tree_mask is not None and tree_seqs is None and query_len_set:
+            longest = max(int(x) for x in query_len_set)
+            if longest > 64 * self.tree_mask.shape[1]:
+                raise ValueError(f"a tree of {longest} tokens needs {-(-longest // 64)} mask words, got {self.tree_mask.shape[1]}")
+        self.window, self.sinks = int(sliding_window or 0), int(sink_tokens)
+        self.queries = queries.contiguous()
+        if self.queries.data_ptr() % 16:
+            self.queries = self.queries.clone()  # a view into the middle of a row: the tensor core's copies start on 16 bytes
+        self.out: torch.Tensor | None = None
+        if self.total == 0:
+            return
+        self.key_cache, self.value_cache = key_cache, value_cache
+        self.scales = (k_scale, v_scale, k_bias, v_bias)
+        self.pool, _ = _make_pool(key_cache, value_cache, self.d, k_scale, v_scale, k_bias, v_bias)
+        tiled_ok = False
+        if kernel == "tiled" and not tiled_ok:
+            raise NotImplementedError(
+                "the tiled kernels need page size 128 (or 16/32/64 with a 16-bit pool), head_dim 64 or 128, fp16/bf16 queries and a pool of "
+                "the same dtype (or an affine pool)")
+        self.kernel = kernel or ("tiled" if tiled_ok else "generic")
+        self.visibility = native_visibility(self.sinks, self.tree_mask, self.tree_seqs)
+        self.status = _scratch.get(dev, "status", 4, zero=True)
+        a = nv.AttnArgs()
+        a.queries = self.queries.data_ptr()
+        a.block_tables, a.kv_lens = self.block_tables.data_ptr(), self.kv_lens.data_ptr()
+        a.query_start_loc = self.query_start_loc.data_ptr()
+        a.total_tokens, a.num_seqs, a.num_q_heads = self.total, self.num_seqs, self.hq
+        a.max_blocks_per_seq, a.q_dtype = int(self.block_tables.shape[1]), nv.dtype_code(queries.dtype)
+        a.sliding_window = self.window
+        a.softmax_scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(self.d)
+        a.max_query_len = max(0, int(max_query_len))
+        a.status = self.status.data_ptr()
+        self.args = a
+
+    def plan(self) -> "VisibleAttentionCall":
+        return self
+
+    def launch(self) -> torch.Tensor:
+        if self.total == 0:
+            return torch.zeros_like(self.queries)
+        lib = nv.lib()
+        self.out = torch.empty_like(self.queries)
+        if _CHECK:
+            self.out.fill_(float("nan"))  # a row no kernel writes shows up in the caller's checks
+        self.args.out = self.out.data_ptr()
+        with nv.on_device(self.device):
+            nv.check(lib.emlx_attn_visible_generic(self.args, self.pool, self.visibility, nv.stream_ptr(self.device)))
+            if _CHECK and not torch.cuda.is_current_stream_capturing():
+                rc = lib.emlx_read_status(nv.ptr(self.status), nv.stream_ptr(self.device))
+                if rc != nv.EMLX_OK:
+                    self.status.zero_()  # report once
+                nv.check(rc)
+        return self.out
+
+
+__all__ = ("VisibleAttentionCall",)

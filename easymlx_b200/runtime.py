@@ -25,7 +25,8 @@ class AttentionStep:
 
     def __init__(self, cache: PageCacheView, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_lens,
                  slot_ids, *, scale: float | None = None, sliding_window: int | None = None, rewind: bool = True,
-                 gather=None):
+                 gather=None, sink_tokens: int = 0, tree_mask: torch.Tensor | None = None, tree_seqs=None, rope=None,
+                 rope_positions: torch.Tensor | None = None):
         self.cache = cache
         self.q, self.k, self.v = q, k, v
         self.query_lens = tuple(int(x) for x in query_lens)
@@ -35,8 +36,12 @@ class AttentionStep:
         self.gather = gather   # distributed.GatherTarget: KV heads sharded over GPUs, output gathered by the kernels
         self._base_lens = cache.kv_lens.clone()
         single = len(self.query_lens) == q.shape[0] and all(x == 1 for x in self.query_lens)
+        # sinks, draft trees and given rotary positions as in PageMetadata; masks and positions are static device tensors
+        # like q / k / v, overwritten between replays
+        self.rope = rope
         self._meta = PageMetadata(query_start_loc=build_query_start_loc(self.query_lens), slot_ids=self.slot_ids,
-                                  sliding_window=sliding_window, is_single_token_decode=single)
+                                  sliding_window=sliding_window, is_single_token_decode=single, sink_tokens=int(sink_tokens),
+                                  tree_mask=tree_mask, tree_seqs=tree_seqs, rope_positions=rope_positions)
         self._meta_lens = None if single else self.query_lens
         self.out: torch.Tensor | None = None
         self.graph: torch.cuda.CUDAGraph | None = None
@@ -45,7 +50,7 @@ class AttentionStep:
 
     def _eager(self) -> torch.Tensor:
         # rewind: the slots' lengths are left as they were, so the same batch can be replayed
-        _, kc, vc, meta = self.cache.concatenate_to_cache(self.q, self.k, self.v, cache_metadata=self._meta,
+        q, kc, vc, meta = self.cache.concatenate_to_cache(self.q, self.k, self.v, cache_metadata=self._meta, rope=self.rope,
                                                           slot_ids=self.slot_ids, query_lens=self.query_lens,
                                                           advance=not self.rewind)
         if self.gather is not None:
@@ -55,14 +60,15 @@ class AttentionStep:
             if self.cache.is_affine:
                 extra = dict(k_scale=self.cache.k_scales, v_scale=self.cache.v_scales, k_bias=self.cache.k_biases,
                              v_bias=self.cache.v_biases)
-            return paged_attention(self.q, kc, vc, meta.block_tables, meta.kv_lens, meta.query_start_loc,
+            return paged_attention(q, kc, vc, meta.block_tables, meta.kv_lens, meta.query_start_loc,
                                    softmax_scale=self.performer.scale, sliding_window=meta.sliding_window,
                                    single_token_decode=meta.is_single_token_decode,
                                    max_query_len=int(getattr(meta, "max_query_len", 0) or 0),
                                    plan=getattr(meta, "plan", None), query_len_set=getattr(meta, "query_len_set", None),
-                                   gather=self.gather, **extra)
+                                   gather=self.gather, sink_tokens=meta.sink_tokens, tree_mask=meta.tree_mask,
+                                   tree_seqs=meta.tree_seqs, **extra)
         op = self.performer.executor.mixin_impl
-        return op(query=self.q, key=kc, value=vc, cache_metadata=meta, cache_view=self.cache,
+        return op(query=q, key=kc, value=vc, cache_metadata=meta, cache_view=self.cache,
                   scale=self.performer.scale).attention_outputs
 
     def capture(self, warmup: int = 3, steps_per_graph: int = 1) -> "AttentionStep":

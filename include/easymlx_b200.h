@@ -54,7 +54,8 @@ enum {
     EMLX_DEV_BAD_PAGE = 2,        /* page id outside [0, num_blocks) inside a sequence's live range   */
     EMLX_DEV_OVERFLOW = 4,        /* a sequence would outgrow its page-table row                      */
     EMLX_DEV_TOKEN_MISMATCH = 8,  /* sum(query_lens) != total_tokens                                  */
-    EMLX_DEV_WAIT_TIMEOUT = 16    /* an in-kernel barrier wait hit its iteration limit                */
+    EMLX_DEV_WAIT_TIMEOUT = 16,   /* an in-kernel barrier wait hit its iteration limit                */
+    EMLX_DEV_BAD_TREE = 32        /* a tree has more tokens than its mask has bits, or an accepted path is not increasing */
 };
 
 /* The page pool, shared by the write and attention entry points. */
@@ -288,6 +289,105 @@ int emlx_gather_init(void* flag_block, void* const* out_ptrs, void* const* flag_
  * args->out = this rank's full [T, total_q_heads, D] buffer and of every other rank's. */
 int emlx_attn_decode_gather(const emlx_attn_args* args, const emlx_pool* pool, void* flag_block, int32_t total_q_heads,
                             int32_t head_offset, void* stream);
+
+/* ---- rows that see something else than a causal window: sinks and draft trees -------------------------------------
+ * A sequence has ctx = kv_len - q_len keys from earlier steps and q_len new ones.  The visible sequence of row i is the
+ * context followed by the new keys whose mask bit is set, in slot order (causal: every new key up to itself); n_i is the
+ * number of those.  A sliding window W keeps the entries of rank >= ctx + n_i - W, sink_tokens N the entries of rank < N
+ * on top (without a window sinks mean nothing: all keys are visible).  A row that sees no key gets zeros. */
+typedef struct emlx_visibility {
+    const uint64_t* tree_mask;  /* device [T, tree_words]: bit j % 64 of word j / 64 = the row sees new key j of its
+                                 * sequence (itself only when its own bit is set); NULL = causal rows              */
+    const int32_t* tree_seqs;   /* device [S], nonzero: rows of the sequence follow tree_mask, zero: causal rows (a
+                                 * prefill chunk beside the trees); NULL: all sequences are trees                  */
+    int32_t tree_words;         /* 1..64; a tree with more than 64 * tree_words tokens sets EMLX_DEV_BAD_TREE and
+                                 * its further tokens are invisible to the rows                                    */
+    int32_t sink_tokens;
+} emlx_visibility;
+
+/* Coverage kernel for any geometry (head_dim <= 256, any page size, every type); needs neither plan nor workspace. */
+int emlx_attn_visible_generic(const emlx_attn_args* args, const emlx_pool* pool, const emlx_visibility* visibility, void* stream);
+
+/* Work list of an attention call over these rows (built by emlx_positioned_step as well).  It also holds the call's
+ * counters: calls that may overlap on the GPU need lists of their own.  8-byte aligned; tree_words = 0 without a mask. */
+size_t emlx_visible_plan_bytes(int32_t num_seqs, int32_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                               int32_t tree_words);
+int emlx_visible_plan(const int32_t* query_start_loc, const int32_t* kv_lens, int32_t num_seqs, int32_t total_tokens,
+                      int32_t num_q_heads, int32_t num_kv_heads, int32_t block_size, int32_t sliding_window,
+                      const emlx_visibility* visibility, int32_t max_query_len /* host hint, 0 = unknown */,
+                      int32_t plan_flags, void* plan, size_t plan_bytes, int32_t* status, void* stream);
+
+/* ---- cache step with given rotary positions ---------------------------------------------------------------------- */
+/* Where the angles come from: pair i of a head turns by positions[pair_axis[i]][token] * inv_freq[i], the product taken
+ * and reduced in 64 bits.  emlx_rope gives the layout (dims, traditional, mscale); its inv_freq and position_scale are
+ * not read. */
+typedef struct emlx_axes {
+    const int32_t* positions;  /* device [num_axes, T], rows axis_stride apart; NULL: the slot of the token in its
+                                * sequence, or under a tree the context length + visible new keys - 1            */
+    const uint8_t* pair_axis;  /* device [dims / 2], axis of every pair; NULL: axis 0                             */
+    const double* inv_freq;    /* device [dims / 2], the position scale multiplied in                             */
+    int64_t axis_stride;
+    int32_t num_axes;
+    int32_t reserved;
+} emlx_axes;
+
+typedef struct emlx_step_args {  /* as the parameters of emlx_kv_write_step */
+    const void* queries;
+    void* queries_out;             /* with rope: [T, Hq, D] rotated queries, NULL: keys only */
+    const void* keys;
+    const void* values;
+    const int32_t* query_lens;     /* NULL: one token per sequence */
+    const int32_t* slot_ids;
+    const int32_t* block_tables_all;
+    int32_t* kv_lens_all;
+    int32_t* query_start_loc;
+    int32_t* block_tables;
+    int32_t* kv_lens;
+    int32_t* ticket;
+    int32_t* status;
+    void* plan;                    /* NULL, or emlx_visible_plan_bytes() bytes: the work list for emlx_attn_visible */
+    size_t plan_bytes;
+    int32_t in_dtype, num_seqs, total_tokens, num_slots, max_blocks_per_seq, advance_kv_lens;
+    int32_t num_q_heads, sliding_window, max_query_len, plan_flags;
+} emlx_step_args;
+
+/* emlx_kv_write_step with rotary positions from `axes` (rope and axes NULL: no rotation) and a work list for the rows
+ * of `visibility` (NULL: causal rows).  Up to 2048 sequences. */
+int emlx_positioned_step(const emlx_step_args* args, const emlx_pool* pool, const emlx_rope* rope, const emlx_axes* axes,
+                         const emlx_visibility* visibility, void* stream);
+/* The same rows with their pool rows given (slot_mapping and token_positions of emlx_build_metadata; larger batches), or
+ * without a pool: queries [T, Hq, D] rotated into queries_out, rows of rope->head_dim_if_no_pool elements.
+ * query_start_loc / num_seqs are read under a tree only. */
+int emlx_positioned_write(const void* queries, void* queries_out, int32_t num_q_heads, const void* keys, const void* values,
+                          int32_t in_dtype, int32_t total_tokens, const int64_t* slot_mapping, const int32_t* token_positions,
+                          const int32_t* query_start_loc, int32_t num_seqs, const emlx_rope* rope, const emlx_axes* axes,
+                          const emlx_visibility* visibility, const emlx_pool* pool, int32_t* status, void* stream);
+
+/* ---- keeping the accepted path of a tree -------------------------------------------------------------------------- */
+typedef struct emlx_commit_layer {
+    void* key_cache;
+    void* value_cache;
+    void* k_scale;  /* AFFINE only */
+    void* k_bias;
+    void* v_scale;
+    void* v_bias;
+    const int32_t* block_tables;  /* [num_slots, MB] */
+    int32_t* kv_lens;             /* [num_slots], the context lengths before the tree */
+    int64_t num_blocks;
+    int32_t advance;              /* add the path length to kv_lens (once for an array that several layers share) */
+    int32_t reserved;
+} emlx_commit_layer;
+
+/* For every scheduled sequence i with context length c = kv_lens[slot_ids[i]]: the K/V rows of the accepted new tokens
+ * move to the front of the tree, row c + accepted[i, j] to row c + j, and committed[i] = c + path length (of layer 0).
+ *   accepted [S, max_path]   strictly increasing token indices of the tree, ended by -1 or by max_path
+ * A path that is not increasing sets EMLX_DEV_BAD_TREE, a slot out of range or listed twice EMLX_DEV_BAD_SLOT (the first
+ * listing counts), a row outside the table EMLX_DEV_OVERFLOW, a page outside the pool EMLX_DEV_BAD_PAGE; such a
+ * sequence is left alone.  `pool` gives the geometry and format that all layers share (its pointers and num_blocks are
+ * not read).  All layers go in one launch per 32; `ticket` as in emlx_kv_write_step. */
+int emlx_commit_tree(const emlx_commit_layer* layers, int32_t num_layers, const emlx_pool* pool, const int32_t* slot_ids,
+                     int32_t num_seqs, const int32_t* accepted, int32_t max_path, int32_t num_slots,
+                     int32_t max_blocks_per_seq, int32_t* committed, int32_t* ticket, int32_t* status, void* stream);
 
 /* Failure-detection self-test: launches one warp that waits, with the kernels' bounded-wait routine and a limit of
  * `poll_limit` polls, on a barrier that is never completed; the wait gives up, the kernel ORs EMLX_DEV_WAIT_TIMEOUT
