@@ -117,6 +117,8 @@ SIGNATURES = {
     "emlx_visible_plan_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I32]),
     "emlx_visible_plan": (C.c_int, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, C.POINTER(Visibility), _I32, _I32, _P, C.c_size_t,
                                    _P, _P]),
+    "emlx_visible_workspace_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I32]),
+    "emlx_attn_visible": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(Pool), C.POINTER(Visibility), _P]),
     "emlx_positioned_step": (C.c_int, [C.POINTER(StepArgs), C.POINTER(Pool), C.POINTER(Rope), C.POINTER(Axes),
                                       C.POINTER(Visibility), _P]),
     "emlx_positioned_write": (C.c_int, [_P, _P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _I32, C.POINTER(Rope), C.POINTER(Axes),

@@ -36,7 +36,7 @@ __device__ __forceinline__ float2 h2_to_f2(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-template <int D, int NT, int FMT, bool BF16, bool PEER, bool HELP>
+template <int D, int NT, int FMT, bool BF16, bool PEER, bool HELP, bool VIS>
 __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint8_t* stages, uint8_t* fixed,
                                                       uint64_t* full, uint64_t* empty, volatile int* abort_word,
                                                       long long f_begin, long long f_end, long long total_flat,
@@ -106,6 +106,12 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
         const int ntiles = desc->ntiles, cum_u = desc->cum_u;
         const int R = q_len * p.G, ctx = kv_len - q_len;
         const int rows_here = min(ROWS, R - row0);
+        bool tree = false;
+        int sinks_in = 0, key_lo = 0;
+        if constexpr (VIS) {
+            const UnitView view(p, desc->seq, row0, tile_lo, q_len, kv_len);
+            tree = view.tree; sinks_in = view.sinks_in; key_lo = view.lo;
+        }
 
         int row_hi[NT][2], row_lo[NT][2];
 #pragma unroll
@@ -114,15 +120,11 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
             for (int e = 0; e < 2; ++e) {
                 const int rr = min(row0 + 8 * nt + 2 * t + e, R - 1);
                 const int i = rr / p.G;
-                int hi = min(kv_len, ctx + i + 1);
-                int lo = p.window > 0 ? max(0, min(kv_len - 1, ctx + i) - p.window + 1) : 0;
-                if (hi <= 0) { hi = 0; lo = 0; }
-                row_hi[nt][e] = hi;
-                row_lo[nt][e] = lo;
+                row_bounds<VIS>(p, tree, qs, i, q_len, kv_len, row_lo[nt][e], row_hi[nt][e]);
             }
         const int i_first = row0 / p.G, i_last = (row0 + rows_here - 1) / p.G;
-        const int hi_min = min(kv_len, ctx + i_first + 1);
-        const int lo_max = p.window > 0 ? max(0, min(kv_len - 1, ctx + i_last) - p.window + 1) : 0;
+        int lo_max, hi_min;
+        unit_bounds<VIS>(p, tree, i_first, i_last, q_len, kv_len, lo_max, hi_min);
 
         // Q^T fragments (B operand) from the staged rows; rows past the unit's last one are zero
         uint32_t qf[KS][NT][2];
@@ -217,8 +219,8 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
             uint8_t* st = stages + (size_t)stage * C::STAGE;
             const uint32_t st_base = ptx::smem_u32(st);
             const __half* sbs = (const __half*)(st + C::KBYTES + C::VBYTES);
-            const int t0 = (tile_lo + j_first + jj) * kTile;
-            const bool interior = (t0 + kTile <= hi_min) && (t0 >= lo_max);
+            const int t0 = (VIS ? tile_of(j_first + jj, sinks_in, tile_lo) : tile_lo + j_first + jj) * kTile;
+            const bool interior = (t0 + kTile <= hi_min) && (t0 >= lo_max || (VIS && t0 + kTile <= p.vis.sinks));
             ptx::mbar_wait(&full[stage], (it / C::STAGES) & 1, abort_word);
 #ifdef EMLX_TRACE_PARTS
             if (p.trace && tid == 0 && jj == 0) asm volatile("mov.u64 %0, %globaltimer;" : "=l"(trace_d));
@@ -321,15 +323,17 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int tok = t0 + (c < 2 ? tokA : tokB);
-                        if (tok < row_lo[nt][c & 1] || tok >= row_hi[nt][c & 1]) s[nt][c] = -INFINITY;
+                        const int i = VIS ? min(row0 + 8 * nt + 2 * t + (c & 1), R - 1) / p.G : 0;
+                        if (!key_seen<VIS>(p, tree, qs, i, ctx, kv_len, q_len, tok, row_lo[nt][c & 1], row_hi[nt][c & 1])) s[nt][c] = -INFINITY;
                     }
                 if constexpr (FMT == 0) {
-                    // this warp is the only reader of its 16 value rows: clear the ones past the sequence end
-                    if (t0 + kTile > kv_len) {
+                    // this warp is the only reader of its 16 value rows: clear the ones past the sequence end (in the VIS
+                    // builds also those between the sinks and the window)
+                    if (t0 + kTile > kv_len || (VIS && t0 < key_lo && t0 + kTile > p.vis.sinks)) {
                         const int first = max(0, kv_len - t0);
                         for (int c = lane; c < 16 * (D / 8); c += 32) {
                             const int tok = 16 * warp + c / (D / 8), ch = c % (D / 8);
-                            if (tok >= first)
+                            if (tok >= first || (VIS && t0 + tok < key_lo && t0 + tok >= p.vis.sinks))
                                 *(uint4*)(st + C::KBYTES + (ch >> 3) * (kTile * 128) + tok * 128 + (ch & 7) * 16) =
                                     make_uint4(0u, 0u, 0u, 0u);
                         }

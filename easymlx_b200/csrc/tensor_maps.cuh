@@ -14,7 +14,8 @@ EncodeTiledFn encode_fn();
 struct MapPair {
     CUtensorMap k, v;
 };
-// Maps of the pool (cached per pool address and geometry).
+// Maps of the pool: encoded for this call, or cached per pool address and geometry.
+int encode_maps(const emlx_pool& pool, MapPair* out);
 int get_maps(const emlx_pool& pool, MapPair* out);
 // Launches the tcgen05 prefill kernel over the plan's 128-row units.  `queue`: two zero-initialised ints of the
 // workspace (item counter, finished CTAs).  `wait_late`: the launch right before this one in the stream is the
@@ -38,7 +39,9 @@ struct DequantScratch {
     int cap;           // pages: max_blocks_per_seq for each sequence the scratch was sized for
 };
 bool dequant_scratch_layout(const emlx_pool* pool, const emlx_attn_args* a, uint8_t* base, size_t bytes, DequantScratch* out);
-int launch_dequant_pages(const emlx_attn_args* a, const emlx_pool* pool, const DequantScratch& sc, cudaStream_t stream);
+// Pages before `window` of the sequence's first new token are left out, unless they hold one of the first `sinks` tokens.
+int launch_dequant_pages(const emlx_attn_args* a, const emlx_pool* pool, const DequantScratch& sc, cudaStream_t stream, int window,
+                         int sinks);
 int launch_convert_out_rows(const emlx_attn_args* a, const emlx_pool* pool, const DequantScratch& sc, cudaStream_t stream);
 
 }  // namespace emlx

@@ -64,7 +64,13 @@ class VisibleAttentionCall:
         self.key_cache, self.value_cache = key_cache, value_cache
         self.scales = (k_scale, v_scale, k_bias, v_bias)
         self.pool, _ = _make_pool(key_cache, value_cache, self.d, k_scale, v_scale, k_bias, v_bias)
-        tiled_ok = False
+        tiled_ok = (
+            (self.pool.block_size == _TILED_BLOCK_SIZE_AFFINE if affine else self.pool.block_size in _TILED_BLOCK_SIZES_FLOAT)
+            and self.d in _TILED_HEAD_DIMS
+            and queries.dtype in (torch.float16, torch.bfloat16)
+            and (affine or key_cache.dtype == queries.dtype)
+            and (key_cache.data_ptr() | value_cache.data_ptr()) % 16 == 0
+        )
         if kernel == "tiled" and not tiled_ok:
             raise NotImplementedError(
                 "the tiled kernels need page size 128 (or 16/32/64 with a 16-bit pool), head_dim 64 or 128, fp16/bf16 queries and a pool of "
@@ -83,8 +89,40 @@ class VisibleAttentionCall:
         a.max_query_len = max(0, int(max_query_len))
         a.status = self.status.data_ptr()
         self.args = a
+        if self.kernel == "generic":
+            return
+        lib, hkv = nv.lib(), self.pool.num_kv_heads
+        words = 0 if self.tree_mask is None else int(self.tree_mask.shape[1])
+        flags = visible_plan_flags(self.pool.kv_format, self.hq, hkv, self.d, int(long_seqs))
+        self.plan_bytes = int(lib.emlx_visible_plan_bytes(self.num_seqs, self.total, self.hq, hkv, words))
+        self.planned = (isinstance(plan, VisiblePlan) and plan.num_q_heads == self.hq and plan.sliding_window == self.window
+                        and plan.sink_tokens == self.sinks and plan.flags == flags and plan.buffer.numel() >= self.plan_bytes
+                        and plan.tree_mask is self.tree_mask and plan.tree_seqs is self.tree_seqs)
+        self.plan_buf = plan.buffer if self.planned else torch.empty(self.plan_bytes, dtype=torch.uint8, device=dev)
+        a.plan_flags = flags
+        if query_len_set:
+            group, wide = self.hq // hkv, bool(flags & 1)
+            for q_len in query_len_set:
+                rows = int(q_len) * group
+                if rows > 0:
+                    a.row_class_mask |= 1 << (0 if rows <= 8 else 1 if rows <= 16 else (3 if wide else 2))
+        ws_bytes = int(lib.emlx_visible_workspace_bytes(self.hq, hkv, self.d, int(a.max_query_len), flags))
+        if affine and flags & 1:
+            ws_bytes += int(lib.emlx_attn_dequant_bytes(self.pool, self.num_seqs, int(self.block_tables.shape[1]), int(long_seqs),
+                                                        self.total, self.hq, nv.dtype_code(queries.dtype)))
+        self.workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        a.plan, a.plan_bytes = self.plan_buf.data_ptr(), self.plan_bytes
+        a.workspace, a.workspace_bytes = self.workspace.data_ptr(), ws_bytes
 
     def plan(self) -> "VisibleAttentionCall":
+        if self.total and self.kernel != "generic" and not self.planned:
+            with nv.on_device(self.device):
+                nv.check(nv.lib().emlx_visible_plan(
+                    nv.ptr(self.query_start_loc), nv.ptr(self.kv_lens), self.num_seqs, self.total, self.hq,
+                    self.pool.num_kv_heads, self.pool.block_size, self.window, self.visibility, int(self.args.max_query_len),
+                    int(self.args.plan_flags), nv.ptr(self.plan_buf), self.plan_bytes, nv.ptr(self.status),
+                    nv.stream_ptr(self.device)))
+            self.planned = True
         return self
 
     def launch(self) -> torch.Tensor:
@@ -96,7 +134,8 @@ class VisibleAttentionCall:
             self.out.fill_(float("nan"))  # a row no kernel writes shows up in the caller's checks
         self.args.out = self.out.data_ptr()
         with nv.on_device(self.device):
-            nv.check(lib.emlx_attn_visible_generic(self.args, self.pool, self.visibility, nv.stream_ptr(self.device)))
+            entry = lib.emlx_attn_visible_generic if self.kernel == "generic" else lib.emlx_attn_visible
+            nv.check(entry(self.args, self.pool, self.visibility, nv.stream_ptr(self.device)))
             if _CHECK and not torch.cuda.is_current_stream_capturing():
                 rc = lib.emlx_read_status(nv.ptr(self.status), nv.stream_ptr(self.device))
                 if rc != nv.EMLX_OK:

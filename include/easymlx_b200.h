@@ -317,6 +317,14 @@ int emlx_visible_plan(const int32_t* query_start_loc, const int32_t* kv_lens, in
                       const emlx_visibility* visibility, int32_t max_query_len /* host hint, 0 = unknown */,
                       int32_t plan_flags, void* plan, size_t plan_bytes, int32_t* status, void* stream);
 
+/* Attention over these rows with the work list above: short rows as emlx_attn_unified, rows beyond 16 per sequence
+ * (plan_flags bit 0) as 256-row units on the tensor cores whose keys are split over CTAs when there are few of them.
+ * `workspace` needs no zeroing; over an affine pool with plan_flags bit 0, emlx_attn_dequant_bytes() follow
+ * emlx_visible_workspace_bytes(). */
+size_t emlx_visible_workspace_bytes(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_query_len,
+                                    int32_t plan_flags);
+int emlx_attn_visible(const emlx_attn_args* args, const emlx_pool* pool, const emlx_visibility* visibility, void* stream);
+
 /* ---- cache step with given rotary positions ---------------------------------------------------------------------- */
 /* Where the angles come from: pair i of a head turns by positions[pair_axis[i]][token] * inv_freq[i], the product taken
  * and reduced in 64 bits.  emlx_rope gives the layout (dims, traditional, mscale); its inv_freq and position_scale are

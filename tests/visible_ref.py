@@ -56,12 +56,17 @@ class Batch:
             kf = kv_quant.dequantize_key_pool(arrays[0], arrays[2], arrays[3], bits).astype(np.float64)
             vf = kv_quant.dequantize_value_pool(arrays[1], arrays[4], arrays[5], bits).astype(np.float64)
             self.k64, self.v64 = kf, vf
+            # a quantised row is scale * code + bias, and the kernels sum the two products apart: what is rounded (and summed)
+            # is as large as |scale * code| and |bias| are, however small their sum is
+            kb, vb = (np.repeat(a.astype(np.float64).transpose(0, 2, 1, 3), 64, -1) for a in (arrays[3], arrays[5]))
+            self.kabs, self.vabs = np.abs(kf - kb) + np.abs(kb), np.abs(vf - vb) + np.abs(vb)
         else:
             if poison is not None:
                 k[~self.owned] = poison
                 v[~self.owned] = poison
             self.arrays = {"key": k, "value": v}
             self.k64, self.v64 = k.double().numpy(), v.double().numpy()
+            self.kabs, self.vabs = np.abs(self.k64), np.abs(self.v64)
         self.kv_lens = np.asarray(total, np.int32)
         self.qsl = np.concatenate([[0], np.cumsum(qlens)]).astype(np.int32)
         self.mask = self.tree_seqs = None
@@ -79,10 +84,10 @@ class Batch:
                 self.tree_seqs = torch.tensor([p is not None for p in trees])
 
     def rows(self, s):
-        """K and V of sequence ``s`` in slot order, 64 bits, ``[kv_len, Hkv, D]``."""
+        """K and V of sequence ``s`` in slot order, 64 bits, ``[kv_len, Hkv, D]``, and the sizes of what they are summed from."""
         pos = np.arange(int(self.kv_lens[s]))
         at = (self.table[s, pos // self.page], pos % self.page)
-        return self.k64[at], self.v64[at]
+        return self.k64[at], self.v64[at], self.kabs[at], self.vabs[at]
 
     def line(self, s, i, window, sinks):
         """Visible keys of row ``i`` of sequence ``s``, in order."""
@@ -104,7 +109,7 @@ class Batch:
         g = self.hq // self.hkv
         q = self.q.double().numpy()
         for s in range(len(self.ctx)):
-            k, v = self.rows(s)
+            k, v, kabs, vabs = self.rows(s)
             for i in range(self.qlens[s]):
                 keys = self.line(s, i, window, sinks)
                 if not keys:
@@ -114,8 +119,8 @@ class Batch:
                 w = np.exp(sc - sc.max(-1, keepdims=True))
                 w /= w.sum(-1, keepdims=True)
                 out[self.qsl[s] + i] = np.einsum("hgn,nhd->hgd", w, v[keys]).reshape(self.hq, self.d)
-                mass[self.qsl[s] + i] = np.einsum("hgn,nhd->hgd", w, np.abs(v[keys])).reshape(self.hq, self.d)
-                reach[self.qsl[s] + i, :, 0] = (np.einsum("hgd,nhd->hgn", np.abs(row), np.abs(k[keys])).max(-1) * scale).reshape(-1)
+                mass[self.qsl[s] + i] = np.einsum("hgn,nhd->hgd", w, vabs[keys]).reshape(self.hq, self.d)
+                reach[self.qsl[s] + i, :, 0] = (np.einsum("hgd,nhd->hgn", np.abs(row), kabs[keys]).max(-1) * scale).reshape(-1)
         return out, mass, reach
 
     def call(self, scale, window=0, sinks=0, kernel=None, hints=True, **kw):
@@ -136,7 +141,8 @@ def attention_bound(batch, out, mass, reach, expanded=False):
     """Largest error a kernel may have, element by element.
 
     A weight is rounded once to the 16-bit type of the product with V (half a step u of itself, so u * sum w |v| in the
-    sum), the output once more (u |out|).  A score is a 32-bit sum of D products: off by at most D 2^-24 sum |q||k| scale,
+    sum), the output once more (u |out|).  Over a quantised pool v = scale * code + bias: the product of weight and scale is
+    what is rounded, so |v| is replaced by |scale * code| + |bias| there (and |k| likewise in the scores).  A score is a 32-bit sum of D products: off by at most D 2^-24 sum |q||k| scale,
     and a score that is off by e changes every normalised weight by at most a factor 1 + 2e (to first order, numerator and
     denominator).  The exponentials (2^-22) and the 32-bit sums over the keys in blocks (2^-20 allows 16 roundings of the
     running values) come on top.  ``expanded``: rows of a quantised pool that were rounded to fp16 first, which moves a
