@@ -263,6 +263,8 @@ def _own_call(st):
         with torch.cuda.graph(graph):
             rotated = write()
 
+        st["keep"] = (cache, rope, meta)  # the graph reads their tables and lengths
+
         def replay():
             graph.replay()
             return {"q": rotated, "k": st["k"], "v": st["v"]}
