@@ -123,7 +123,7 @@ SIGNATURES = {
                                       C.POINTER(Visibility), _P]),
     "emlx_positioned_write": (C.c_int, [_P, _P, _I32, _P, _P, _I32, _I32, _P, _P, _P, _I32, C.POINTER(Rope), C.POINTER(Axes),
                                        C.POINTER(Visibility), C.POINTER(Pool), _P, _P]),
-    "emlx_commit_tree": (C.c_int, [C.POINTER(CommitLayer), _I32, C.POINTER(Pool), _P, _I32, _P, _I32, _I32, _I32, _P, _P, _P, _P]),
+    "emlx_commit_tree": (C.c_int, [_P, _I32, C.POINTER(Pool), _P, _I32, _P, _I32, _I32, _I32, _P, _P, _P, _P]),
     "emlx_rows_assign": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32, _P]),
     "emlx_rows_update": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32, _P, _P]),
 }

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 import os
+import struct
 import typing as tp
 from collections import OrderedDict
 from dataclasses import dataclass, field
@@ -75,12 +76,15 @@ class _DeviceIntCache:
     def __init__(self, capacity: int = 64):
         self.capacity = capacity
         self.items: OrderedDict = OrderedDict()
+        self.captured: dict = {}  # handed out during a stream capture: the graph reads them for as long as it lives
 
     def get(self, values: tuple[int, ...], device) -> torch.Tensor:
         key = (values, str(device))
         hit = self.items.get(key)
         if hit is not None:
             self.items.move_to_end(key)
+            if hit.is_cuda and torch.cuda.is_current_stream_capturing():
+                self.captured[key] = hit
             return hit
         t = torch.tensor(values, dtype=torch.int32).pin_memory().to(device, non_blocking=True) if values else \
             torch.zeros(0, dtype=torch.int32, device=device)
@@ -271,6 +275,7 @@ class PageCacheView:
         self.cache_bits = int(cache_bits)
         self._status: torch.Tensor | None = None
         self._ticket: torch.Tensor | None = None
+        self._commit: tuple | None = None
         self._validate_shape()
 
     # ------------------------------------------------------------------ geometry
@@ -397,14 +402,25 @@ class PageCacheView:
             raise IndexError(f"Invalid seq_idx {seq_idx}")
         return int(self.kv_lens[seq_idx].item()) + int(num_new_tokens) <= self.max_seq_len
 
-    def _commit_geometry(self) -> tuple:
-        for t in (self.block_tables, self.kv_lens):
+    def _commit_row(self) -> tuple:
+        """``(descriptor bytes, geometry, pool)`` of this layer for ``emlx_commit_tree``; made again when a tensor or its
+        memory is another one than last time."""
+        kc, vc, bt, lens = self.key_cache, self.value_cache, self.block_tables, self.kv_lens
+        at = (kc.data_ptr(), vc.data_ptr(), bt.data_ptr(), lens.data_ptr())
+        row = self._commit
+        if row is not None and row[3] == at and row[4] is kc and row[5] is vc and row[6] is bt and row[7] is lens:
+            return row
+        for t in (bt, lens):
             if t.dtype != torch.int32 or not t.is_contiguous():
                 raise ValueError("block_tables and kv_lens must be contiguous int32")
-        if not (self.key_cache.is_contiguous() and self.value_cache.is_contiguous()):
+        if not (kc.is_contiguous() and vc.is_contiguous()):
             raise ValueError("key_cache and value_cache must be contiguous")
-        return (self.block_size, self.num_kv_heads, self.head_dim, self.cache_bits, self.key_cache.dtype, self.num_seqs,
-                self.blocks_per_seq, self.key_cache.device)
+        pool = self.native_pool()
+        words = [pool.key_cache, pool.value_cache, pool.k_scale, pool.k_bias, pool.v_scale, pool.v_bias, at[2], at[3], pool.num_blocks]
+        geometry = (self.block_size, self.num_kv_heads, self.head_dim, self.cache_bits, kc.dtype, self.num_seqs, self.blocks_per_seq,
+                    kc.device)
+        self._commit = row = (struct.pack("9q", *(int(w or 0) for w in words)), geometry, pool, at, kc, vc, bt, lens)
+        return row
 
     # ------------------------------------------------------------------ native descriptors
     def native_pool(self) -> nv.Pool:
@@ -503,7 +519,7 @@ class PageCacheView:
         return qsl, bt, lens, (None if plan is None else (plan, hq, window, flags)), rotated_q
 
     def _write_positioned(self, keys, values, query_lens_dev, slots_dev, total: int, queries, *, rope, positions, window: int,
-                          max_q: int, long_seqs: int, advance: bool, sinks: int, tree_mask, tree_seqs):
+                          max_q: int, long_seqs: int, advance: bool, sinks: int, tree_mask, tree_seqs, query_lens=None):
         """``_write_batch`` for a step with sinks, a draft tree or given rotary positions (``query_lens_dev`` ``None``: one
         token per sequence): the rows, the metadata and the work list of ``visible_attention`` in one launch."""
         nv.require_cuda(keys, values, queries, self.key_cache)
@@ -547,6 +563,8 @@ class PageCacheView:
         if visible and total > 0 and hq % self.num_kv_heads == 0 and (
                 self.block_size == 128 or (not self.is_affine and self.block_size in (16, 32, 64))):
             flags = visible_plan_flags(self.cache_bits if self.is_affine else 0, hq, self.num_kv_heads, self.head_dim, long_seqs)
+            if query_lens:
+                flags |= absent_row_classes(set(query_lens), hq // self.num_kv_heads, bool(flags & 1))
             plan_bytes = int(lib.emlx_visible_plan_bytes(s, total, hq, self.num_kv_heads, words))
             plan = torch.empty(plan_bytes, dtype=torch.uint8, device=dev)
         with nv.on_device(dev):
@@ -779,7 +797,7 @@ class PageCacheView:
             qsl, bt, lens, plan, rotated_q, keep = self._write_positioned(
                 keys, values, None if single and len(slots) == total else qlens_dev, _uploaded.get(slots, dev), total,
                 queries, rope=rope, positions=positions, window=window, max_q=max_q, long_seqs=long_seqs, advance=advance,
-                sinks=sinks, tree_mask=tree_mask, tree_seqs=tree_seqs)
+                sinks=sinks, tree_mask=tree_mask, tree_seqs=tree_seqs, query_lens=qlens)
             if rotated_q is not None:
                 queries = rotated_q
             meta = PageMetadata(
@@ -815,22 +833,29 @@ def visible_plan_flags(bits: int, num_q_heads: int, num_kv_heads: int, head_dim:
     return flags
 
 
+def absent_row_classes(query_lens: tp.Iterable[int], group: int, wide: bool) -> int:
+    """Plan flags of the row classes that do not occur among the query lengths (bits 16 to 19); 0 when nothing is known."""
+    seen = 0
+    for q_len in query_lens:
+        rows = int(q_len) * group
+        if rows > 0:
+            seen |= 1 << (0 if rows <= 8 else 1 if rows <= 16 else (3 if wide else 2))
+    return (~seen & 15) << 16 if seen else 0
+
+
 def commit_layers(views: tp.Sequence[PageCacheView], slot_ids, accepted, *, advance: bool = True) -> torch.Tensor:
     """The launch behind every ``commit_tree``: the views are the layers of one cache, alike in geometry and format."""
     if not views:
         raise ValueError("commit_tree needs at least one layer")
     first = views[0]
-    dev, geometry = first.key_cache.device, first._commit_geometry()
-    layers = (nv.CommitLayer * len(views))()
-    for layer, view in zip(layers, views):
-        if view is not first and view._commit_geometry() != geometry:
+    dev = first.key_cache.device
+    rows = [view._commit_row() for view in views]
+    geometry = rows[0][1]
+    for row in rows:
+        if row[1] is not geometry and row[1] != geometry:
             raise ValueError("commit_tree needs layers of the same geometry, format and device")
-        layer.key_cache, layer.value_cache = view.key_cache.data_ptr(), view.value_cache.data_ptr()
-        if view.is_affine:
-            layer.k_scale, layer.k_bias = view.k_scales.data_ptr(), view.k_biases.data_ptr()
-            layer.v_scale, layer.v_bias = view.v_scales.data_ptr(), view.v_biases.data_ptr()
-        layer.block_tables, layer.kv_lens = view.block_tables.data_ptr(), view.kv_lens.data_ptr()
-        layer.num_blocks, layer.advance = view.num_blocks, int(bool(advance))
+    flag = b"\1\0\0\0\0\0\0\0" if advance else b"\0\0\0\0\0\0\0\0"
+    layers = b"".join([part for row in rows for part in (row[0], flag)])
     nv.require_cuda(first.key_cache)
     if isinstance(slot_ids, torch.Tensor):
         if slot_ids.ndim != 1 or slot_ids.dtype.is_floating_point:
@@ -845,11 +870,11 @@ def commit_layers(views: tp.Sequence[PageCacheView], slot_ids, accepted, *, adva
         slots = _uploaded.get(host, dev)
     s = int(slots.shape[0])
     if not isinstance(accepted, torch.Tensor):
-        rows = [[int(x) for x in row] for row in accepted]
-        width = max((len(row) for row in rows), default=0)
-        if any(b <= a for row in rows for a, b in zip([-1] + row[:-1], row)):
+        paths = [[int(x) for x in path] for path in accepted]
+        width = max((len(path) for path in paths), default=0)
+        if any(b <= a for path in paths for a, b in zip([-1] + path[:-1], path)):
             raise ValueError("an accepted path lists token indices in increasing order")
-        accepted = torch.tensor([row + [-1] * (width - len(row)) for row in rows], dtype=torch.int32).reshape(len(rows), width)
+        accepted = torch.tensor([path + [-1] * (width - len(path)) for path in paths], dtype=torch.int32).reshape(len(paths), width)
     if accepted.ndim != 2 or accepted.shape[0] != s or accepted.dtype.is_floating_point:
         raise ValueError(f"accepted must be integers [{s}, max_path], ended by -1")
     if accepted.is_cuda and accepted.device != dev:
@@ -859,7 +884,7 @@ def commit_layers(views: tp.Sequence[PageCacheView], slot_ids, accepted, *, adva
     if s == 0:
         return committed
     with nv.on_device(dev):
-        nv.check(nv.lib().emlx_commit_tree(layers, len(views), first.native_pool(), nv.ptr(slots), s, nv.ptr(accepted),
+        nv.check(nv.lib().emlx_commit_tree(layers, len(views), rows[0][2], nv.ptr(slots), s, nv.ptr(accepted),
                                            int(accepted.shape[1]), first.num_seqs, first.blocks_per_seq, nv.ptr(committed),
                                            nv.ptr(first.ticket), nv.ptr(first.status), nv.stream_ptr(dev)))
     if _CHECK and not torch.cuda.is_current_stream_capturing():

@@ -18,7 +18,9 @@
 // keys as two words (window, sinks, shifted tree mask) and tests constant bits.  Values at tokens that no row of the
 // unit sees are cleared in shared memory first, since 0 * NaN would reach the rows.
 //
-// Warp roles: 0-3 stream 0, 4-7 stream 1, 8 TMA producer, 9 MMA issuer (and TMEM owner), 10-11 idle.  All waits are bounded.
+// Warp roles: 0-3 stream 0, 4-7 stream 1, 8 TMA producer, 9 and 10 MMA issuers of the two
+// streams (9 owns the TMEM), 11 idle.  An issuing warp is held up until the tensor pipe has room for its instructions; with
+// a warp of its own, a stream's products are in the queue as soon as its weights are there.  All waits are bounded.
 #include "tcgen05.cuh"
 #include "tensor_maps.cuh"
 #include "visible_plan.cuh"
@@ -26,8 +28,8 @@
 namespace emlx {
 
 constexpr int kWdSoftThreads = 256;
-constexpr int kWdProducer = 8, kWdMma = 9;
-constexpr int kWdThreads = kWdSoftThreads + 128;  // whole warpgroups, since registers are moved between them (two warps idle)
+constexpr int kWdProducer = 8, kWdMma = 9;  // warps 9 and 10 issue the products of stream 0 and 1
+constexpr int kWdThreads = kWdSoftThreads + 128;  // whole warpgroups, since registers are moved between them (one warp idle)
 // A softmax thread holds a row's 128 scores: it gets the registers that the copying and issuing warps do not need.
 // Together they stay inside what the block is launched with, 168 x 384.
 constexpr int kWdSoftRegs = 216, kWdOtherRegs = 72;
@@ -57,20 +59,25 @@ struct WdCfg {
     static constexpr int QBLOCK = kRowBlock * D * 2;      // one row block of Q
     static constexpr int TILE = kTile * D * 2;            // one K or V tile
     static constexpr int OFF_RING = 2 * QBLOCK;
-    static constexpr int SLOTS = D == 128 ? 5 : 8;
-    static constexpr int OFF_BAR = OFF_RING + SLOTS * TILE;
+    // Ring of tile places, each a K and a V slot: tile t of an item lies in place t % PLACES.  PLACES is even, so that where the
+    // streams take alternate tiles a place belongs to one of them, and whoever waits for a place has seen its every use.
+    static constexpr int PLACES = D == 128 ? 2 : 4;
+    static constexpr int OFF_BAR = OFF_RING + 2 * PLACES * TILE;
     static constexpr int SMEM = OFF_BAR + 512 + 1024;
     static constexpr size_t SLOT_FLOATS = (size_t)kWideRows * (D + 2);
 };
 
 struct WdBarriers {
-    uint64_t full[8], empty[8];     // ring slots
+    uint64_t full[8], empty[8];     // ring slots: 2 j = K of place j, 2 j + 1 = V
     uint64_t q_full, q_free;        // Q loaded; every QK of the item has read it
-    uint64_t s_full[2], p_ready[2]; // per stream: S complete (and with it every earlier product), P written
+    uint64_t s_full[2];             // per stream: S complete (and with it every earlier product)
+    uint64_t p_half[2], p_ready[2]; // per stream: P of the tile's first 64 keys written, all of P written
     uint64_t o_full[2];             // per stream: the item's last PV is complete
     uint64_t item_full[4];
     uint64_t item_done;             // the item's rows are stored
     uint64_t xch;                   // exchange steps between the streams
+    uint64_t turn[2];               // the tensor pipe is stream s's
+    uint64_t drain;                 // every product of the CTA is complete
     int item_ring[4];
     uint32_t tmem_base;
     int abort_word;
@@ -93,15 +100,122 @@ __device__ __forceinline__ WideItem wide_item(const WideParams& p, int idx) {
     it.slot = p.plan[p.L.entry_slot + e] + it.head * it.parts;
     return it;
 }
-// Place of tile t's K and V in the item's load order: the order in which the products use them up.
-__device__ __forceinline__ int k_place(int t, bool pair) { return pair ? 2 * t : (t == 0 ? 0 : 2 * t - 1); }
-__device__ __forceinline__ int v_place(int t, bool pair, int count) { return pair ? 2 * t + 1 : min(2 * t + 2, 2 * count - 1); }
+// Uses of the ring's places so far: every role counts them the same way, item by item.
+template <int PLACES>
+struct RingCount {
+    uint32_t used[PLACES];
+    __device__ __forceinline__ RingCount() {
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) used[j] = 0;
+    }
+    __device__ __forceinline__ uint32_t use_of(int t) const {  // which use of its place tile t of the current item is
+        uint32_t u = used[0];
+#pragma unroll
+        for (int j = 1; j < PLACES; ++j) u = (t % PLACES) == j ? used[j] : u;
+        return u + (uint32_t)(t / PLACES);
+    }
+    __device__ __forceinline__ void finish(int count) {
+#pragma unroll
+        for (int j = 0; j < PLACES; ++j) used[j] += (uint32_t)((count - j + PLACES - 1) / PLACES);
+    }
+};
 
 // Bits [from, to) of the 64 keys that start at `base`.
 __device__ __forceinline__ uint64_t key_range(int from, int to, int base) {
     const int a = max(from - base, 0), b = min(to - base, 64);
     if (b <= a) return 0;
     return (b >= 64 ? ~0ull : (1ull << b) - 1) & ~((1ull << a) - 1);
+}
+
+// 2^x on the special-function unit; ex2(-inf) = 0
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// sm_100's packed and three-operand forms: two 32-bit elements per instruction
+__device__ __forceinline__ uint64_t pack2u(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
+__device__ __forceinline__ uint64_t pack2f(float lo, float hi) { return pack2u(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of two elements on the FMA pipe: x = n + f with |f| <= 1/2, a polynomial of degree 4 in f (coefficients from a weighted
+// least-squares iteration towards equal relative error, 2^-18.4, with 2^0 = 1 exactly) and n added to the exponent.
+// Below -127 the result is 0.  Every kPolyPeriod-th pair of weights is made this way: the special-function unit would
+// need 1024 cycles for the 128 x 128 weights of a stream's tile, which nothing else covers while the other stream's
+// products run.
+constexpr int kPolyPeriod = 8;
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+    float lo, hi;  // (a score that is not a number stays one, so that its row does not come out finite)
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(lo) : "f"(__uint_as_float((uint32_t)x)), "f"(-127.0f));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(hi) : "f"(__uint_as_float((uint32_t)(x >> 32))), "f"(-127.0f));
+    x = pack2f(lo, hi);
+    const uint64_t magic = pack2f(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are the nearest integer
+    const uint64_t t = add2(x, magic);
+    const uint64_t f = fma2(add2(t, pack2f(-12582912.0f, -12582912.0f)), pack2f(-1.0f, -1.0f), x);
+    uint64_t y = pack2f(0x1.3a02ccp-7f, 0x1.3a02ccp-7f);
+    y = fma2(y, f, pack2f(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
+    y = fma2(y, f, pack2f(0x1.ec0378p-3f, 0x1.ec0378p-3f));
+    y = fma2(y, f, pack2f(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+    y = fma2(y, f, pack2f(1.0f, 1.0f));
+    return pack2u((uint32_t)y + ((uint32_t)t << 23), (uint32_t)(y >> 32) + ((uint32_t)(t >> 32) << 23));
+}
+// Waits, with a limit, until a barrier has no copy in flight: until the phase that is open completes, if bytes are
+// expected in it.
+__device__ __forceinline__ void drain_copies(uint64_t* bar) {
+    int never = 0;
+    for (uint32_t parity = 0; parity < 2; ++parity) {
+        if (ptx::mbar_try_wait(bar, parity)) continue;      // the open phase has the other parity
+        ptx::mbar_wait(bar, parity, &never, 1u << 14);      // no copy: the wait runs out
+    }
+}
+// The rare paths stay out of the tile loop's instruction stream: a warp runs through that loop's straight code once per
+// tile, and what lies between costs fetches even when it is skipped.
+//
+// Scores of this thread's row that it does not see become -inf: `seen_at(key)` gives the visibility of the 64 keys from
+// `key` on.
+template <typename F>
+__device__ __forceinline__ void mask_scores(uint32_t s_addr, F seen_at, int t0) {
+#pragma unroll 1
+    for (int w = 0; w < 2; ++w) {
+        const uint64_t seen = seen_at(t0 + 64 * w);
+        if (__all_sync(0xffffffffu, seen == ~0ull)) continue;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t bits = c ? (uint32_t)(seen >> 32) : (uint32_t)seen;
+            uint32_t v[32];
+            tmem_ld32_nowait(s_addr + 64 * w + 32 * c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (!(bits & (1u << e))) v[e] = 0xff800000u;  // -inf
+            tmem_st32_nowait(s_addr + 64 * w + 32 * c, v);
+        }
+    }
+    tmem_wait_st();
+}
+__device__ __forceinline__ void scale_columns(uint32_t addr, int chunks, float factor) {
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+        uint32_t v[32];
+        tmem_ld32_nowait(addr + 32 * c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * factor);
+        tmem_st32_nowait(addr + 32 * c, v);
+    }
 }
 
 template <int D, bool BF16>
@@ -118,20 +232,23 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int s = 0; s < C::SLOTS; ++s) {
+        for (int s = 0; s < 2 * C::PLACES; ++s) {
             ptx::mbar_init(&bars->full[s], 1);
-            ptx::mbar_init(&bars->empty[s], 1);
+            ptx::mbar_init(&bars->empty[s], 2);  // two arrivals per use: one per stream, or both from the one that used it
         }
         ptx::mbar_init(&bars->q_full, 1);
-        ptx::mbar_init(&bars->q_free, 1);
+        ptx::mbar_init(&bars->q_free, 2);  // one per stream
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(&bars->s_full[s], 1);
+            ptx::mbar_init(&bars->p_half[s], kRowBlock);
             ptx::mbar_init(&bars->p_ready[s], kRowBlock);
             ptx::mbar_init(&bars->o_full[s], 1);
+            ptx::mbar_init(&bars->turn[s], 1);
         }
         for (int s = 0; s < 4; ++s) ptx::mbar_init(&bars->item_full[s], 1);
         ptx::mbar_init(&bars->item_done, kWdSoftThreads);
         ptx::mbar_init(&bars->xch, kWdSoftThreads);
+        ptx::mbar_init(&bars->drain, 2);
         bars->abort_word = 0;
         ptx::fence_barrier_init();
         ptx::prefetch_tensormap(&qmap);
@@ -157,7 +274,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         if (warp == kWdProducer) {
             // ------------------------------------------------------------------ TMA producer
             const uint64_t keep = ptx::l2_policy_evict_normal();
-            uint32_t base = 0;  // ring places handed out so far
+            RingCount<C::PLACES> uses;
             uint32_t done_seen = 0;
             int next = lane == 0 ? atomicAdd(queue, 1) : 0;
             bool last_pair = false;
@@ -203,18 +320,18 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 };
                 int pg_cur = load_pages(0), pg_next = load_pages(per_batch), pg_base = 0;
                 auto issue = [&](int t, bool is_k) {
-                    const uint32_t place = base + (uint32_t)(is_k ? k_place(t, pair) : v_place(t, pair, it.count));
-                    const uint32_t slot = place % C::SLOTS, use = place / C::SLOTS;
+                    const uint32_t slot = 2 * (t % C::PLACES) + (is_k ? 0 : 1), use = uses.use_of(t);
                     if (use > 0) ptx::mbar_wait(&bars->empty[slot], (use - 1) & 1, abort_word);
-                    const bool go = lane == 0 && !*abort_word;
-                    if (go) ptx::mbar_arrive_expect_tx(&bars->full[slot], C::TILE);
+                    const bool go = !*abort_word;
+                    if (go && lane == 0) ptx::mbar_arrive_expect_tx(&bars->full[slot], C::TILE);
+                    __syncwarp();
                     uint8_t* tile = ring + (size_t)slot * C::TILE;
                     const long long tok = (long long)tile_of(it.j0 + t, sinks_in, tile_lo) * kTile;
                     for (int sub = 0; sub < ppt; ++sub) {
                         const int at = ((t - pg_base) << ppt_log) + sub;
                         const int a = __shfl_sync(0xffffffffu, pg_cur, at & 31), b = __shfl_sync(0xffffffffu, pg_next, at & 31);
                         const int pg = at < 32 ? a : b;
-                        if (go) {
+                        if (go && elect_one()) {
                             const bool bad = pg < 0 || pg >= p.num_blocks;
                             const long long key = tok + (long long)sub * p.bs;
                             // a page that no row of the unit sees may be gone; a missing one reads as zero rows
@@ -228,28 +345,36 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     }
                     __syncwarp();
                 };
-                // in the order of k_place / v_place
-                if (!pair) issue(0, true);
+                // K runs a ring ahead of V: its slot is free behind QK, V's only behind PV
+                for (int t = 0; t < min(C::PLACES, it.count); ++t) issue(t, true);
                 for (int t = 0; t < it.count; ++t) {
-                    if (pair) issue(t, true);
-                    else if (t + 1 < it.count) issue(t + 1, true);
                     issue(t, false);
-                    if (t + 1 == pg_base + per_batch) {  // tiles below are all issued; at most one tile above is looked up
+                    if (t + C::PLACES < it.count) issue(t + C::PLACES, true);
+                    if (t + 1 == pg_base + per_batch) {  // V below is all issued, and K at most PLACES <= per_batch tiles above
                         pg_base += per_batch;
                         pg_cur = pg_next;
                         pg_next = load_pages(pg_base + per_batch);
                     }
                 }
-                base += 2u * (uint32_t)it.count;
+                uses.finish(it.count);
             }
-        } else if (warp == kWdMma) {
-            // ------------------------------------------------------------------ MMA issuer
+            if (*abort_word) {
+                // a wait of this CTA gave up: its copies in flight must land before the block may leave
+                __threadfence_block();
+                for (int t = 0; t < 2 * C::PLACES; ++t) drain_copies(&bars->full[t]);
+                drain_copies(&bars->q_full);
+            }
+        } else if (warp < kWdMma + 2) {
+            // ------------------------------------------------------------------ MMA issuer of stream s
+            const int s = warp - kWdMma;
             constexpr uint32_t idesc_qk = instr_desc(128, 128, BF16, false);
             constexpr uint32_t idesc_pv = instr_desc(128, D, BF16, true);
             const uint64_t q_desc0 = smem_desc(ptx::smem_u32(q_smem), 16, 1024);
             const uint64_t k_desc0 = smem_desc(ptx::smem_u32(ring), 16, 1024);
             const uint64_t v_desc0 = smem_desc(ptx::smem_u32(ring), kTile * 128, 1024);
-            uint32_t base = 0, p_phase[2] = {0, 0};
+            const uint32_t tS = tmem_S + 128 * s, tO = tmem_O + 128 * s;
+            uint32_t p_phase = 0, t_phase = 0;
+            RingCount<C::PLACES> uses;
             for (uint32_t k = 0;; ++k) {
                 if (!ptx::mbar_wait(&bars->item_full[k & 3], (k >> 2) & 1, abort_word)) break;
                 const int idx = bars->item_ring[k & 3];
@@ -257,52 +382,70 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 const WideItem it = wide_item(p, idx);
                 const int seq = unit_seq[it.u], row0 = unit_row0[it.u];
                 const bool pair = (p.qsl[seq + 1] - p.qsl[seq]) * p.G - row0 > kRowBlock;
-                const int steps = pair ? 2 * it.count : it.count;
+                const int steps = pair ? it.count : (it.count - s + 1) / 2, other = pair ? it.count : (it.count - (s ^ 1) + 1) / 2;
                 ptx::mbar_wait(&bars->q_full, k & 1, abort_word);
-                // S of step n is overwritten by QK of step n + 2 of the same stream: its softmax has arrived on p_ready by then,
-                // and PV of step n, which reads P from the same columns, was issued before (the pipe runs in issue order)
-                auto issue_qk = [&](int n) {
-                    const int s = n & 1, t = pair ? n >> 1 : n;
-                    const uint32_t place = base + (uint32_t)k_place(t, pair), slot = place % C::SLOTS;
-                    const bool ok = ptx::mbar_wait(&bars->full[slot], (place / C::SLOTS) & 1, abort_word);
+                if (steps == 0 && lane == 0) ptx::mbar_arrive(&bars->q_free);
+                // S of step i is overwritten by QK of step i + 1: its softmax has arrived on p_ready by then, and PV of step i,
+                // which reads P from the same columns, was issued before (the pipe runs a thread's products in issue order)
+                auto issue_qk = [&](int i) {
+                    const int t = pair ? i : 2 * i + s;
+                    const uint32_t slot = 2 * (t % C::PLACES);
+                    const bool ok = ptx::mbar_wait(&bars->full[slot], uses.use_of(t) & 1, abort_word);
                     tc_fence_after();
-                    if (lane == 0 && ok) {
+                    if (ok && elect_one()) {
                         const uint64_t qd = q_desc0 + (uint64_t)((pair ? s : 0) * (C::QBLOCK >> 4));
                         const uint64_t kd = k_desc0 + (uint64_t)(slot * (C::TILE >> 4));
-    #pragma unroll
+#pragma unroll
                         for (int ks = 0; ks < D / 16; ++ks) {
                             const uint32_t off = (uint32_t)((ks >> 2) * ((kTile * 128) >> 4) + (ks & 3) * 2);
-                            tc_mma_f16(tmem_S + 128 * s, qd + off, kd + off, idesc_qk, ks > 0);
+                            tc_mma_f16(tS, qd + off, kd + off, idesc_qk, ks > 0);
                         }
                         tc_commit(&bars->s_full[s]);
-                        if (!pair || s == 1) tc_commit(&bars->empty[slot]);
-                        if (n == steps - 1) tc_commit(&bars->q_free);
+                        tc_commit(&bars->empty[slot]);
+                        if (!pair) tc_commit(&bars->empty[slot]);
+                        if (i == steps - 1) tc_commit(&bars->q_free);
                     }
                     __syncwarp();
                 };
-                issue_qk(0);
-                if (steps > 1) issue_qk(1);
-                for (int n = 0; n < steps; ++n) {
-                    const int s = n & 1, t = pair ? n >> 1 : n;
-                    const uint32_t place = base + (uint32_t)v_place(t, pair, it.count), slot = place % C::SLOTS;
-                    bool ok = ptx::mbar_wait(&bars->full[slot], (place / C::SLOTS) & 1, abort_word);
-                    ok = ptx::mbar_wait(&bars->p_ready[s], p_phase[s] & 1, abort_word) && ok;
-                    ++p_phase[s];
-                    tc_fence_after();
-                    if (lane == 0 && ok) {
-                        const uint64_t vd = v_desc0 + (uint64_t)(slot * (C::TILE >> 4));
-    #pragma unroll
-                        for (int kk = 0; kk < kTile / 16; ++kk)
-                            tc_mma_f16_ts(tmem_O + 128 * s, tmem_S + 128 * s + kk * 8, vd + (uint64_t)(kk * ((16 * 128) >> 4)), idesc_pv,
-                                          n > 1 || kk > 0);
-                        if (!pair || s == 1) tc_commit(&bars->empty[slot]);
-                        if (n + 2 >= steps) tc_commit(&bars->o_full[s]);
+                if (steps > 0) issue_qk(0);
+                for (int i = 0; i < steps; ++i, ++p_phase) {
+                    const int t = pair ? i : 2 * i + s;
+                    const uint32_t slot = 2 * (t % C::PLACES) + 1;
+                    bool ok = ptx::mbar_wait(&bars->full[slot], uses.use_of(t) & 1, abort_word);
+                    const uint64_t vd = v_desc0 + (uint64_t)(slot * (C::TILE >> 4));
+                    // The product starts on the first 64 keys while the softmax warps are at the others.  The rest, and QK behind
+                    // it, go in turn with the other stream: two streams that are in step would share the pipe and then the
+                    // special-function unit, one of the two always idle.
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (half == 1 && (s == 1 || i > 0)) {
+                            ptx::mbar_wait(&bars->turn[s], t_phase & 1, abort_word);
+                            ++t_phase;
+                        }
+                        ok = ptx::mbar_wait(half ? &bars->p_ready[s] : &bars->p_half[s], p_phase & 1, abort_word) && ok;
+                        tc_fence_after();
+                        if (ok && elect_one()) {
+#pragma unroll
+                            for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                                tc_mma_f16_ts(tO, tS + kk * 8, vd + (uint64_t)(kk * ((16 * 128) >> 4)), idesc_pv, i > 0 || kk > 0);
+                            if (half == 1) {
+                                tc_commit(&bars->empty[slot]);
+                                if (!pair) tc_commit(&bars->empty[slot]);
+                                if (i == steps - 1) tc_commit(&bars->o_full[s]);
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    if (n + 2 < steps) issue_qk(n + 2);
+                    if (i + 1 < steps) issue_qk(i + 1);
+                    // stream 0 goes first and has as many steps or one more: a turn is given only where it will be taken
+                    if (lane == 0 && (s == 0 ? i < other : i + 1 < other)) ptx::mbar_arrive(&bars->turn[s ^ 1]);
                 }
-                base += 2u * (uint32_t)it.count;
+                uses.finish(it.count);
             }
+            if (elect_one()) tc_commit(&bars->drain);
+            __syncwarp();
+            int never = 0;  // (waited for even when another wait has given up)
+            ptx::mbar_wait(&bars->drain, 0, &never);
         }
     } else {
         // ------------------------------------------------------------------ softmax: thread = row of stream g
@@ -310,7 +453,8 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         const int g = warp >> 2, r = tid & 127;
         const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem_S + 128 * g + lane_addr, o_addr = tmem_O + 128 * g + lane_addr;
-        uint32_t base = 0, s_phase = 0, o_phase[2] = {0, 0}, x_phase = 0;
+        uint32_t s_phase = 0, o_phase[2] = {0, 0}, x_phase = 0;
+        RingCount<C::PLACES> uses;
         auto exchange = [&]() {  // every softmax thread: what was written before is visible behind it
             ptx::mbar_arrive(&bars->xch);
             ptx::mbar_wait(&bars->xch, x_phase & 1, abort_word);
@@ -350,86 +494,11 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 ptx::mbar_wait(&bars->s_full[g], s_phase & 1, abort_word);
                 ++s_phase;
                 tc_fence_after();
-                if (!dead) {
-                    uint32_t sv[kTile];
-#pragma unroll
-                    for (int c = 0; c < kTile / 32; ++c) tmem_ld32_nowait(s_addr + 32 * c, sv + 32 * c);
-                    tmem_wait_ld();
-                    if (!whole) {
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const int b = t0 + 64 * w;
-                            uint64_t seen = key_range(lo, hi, b) | key_range(0, min(sinks, hi), b);
-                            if (tree && b + 64 > ctx && b < kv_len) {
-                                const int j = b - ctx;  // new token that key b is
-                                if (j >= 0) {
-                                    seen |= tree_word(p.vis, bits, j >> 6, q_len) >> (j & 63);
-                                    if (j & 63) seen |= tree_word(p.vis, bits, (j >> 6) + 1, q_len) << (64 - (j & 63));
-                                } else if (j > -64) {
-                                    seen |= tree_word(p.vis, bits, 0, q_len) << (-j);
-                                }
-                            }
-                            const uint32_t s0 = (uint32_t)seen, s1 = (uint32_t)(seen >> 32);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                if (!(s0 & (1u << e))) sv[64 * w + e] = 0xff800000u;  // -inf
-                                if (!(s1 & (1u << e))) sv[64 * w + 32 + e] = 0xff800000u;
-                            }
-                        }
-                    }
-                    float mx8[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(sv[e]);
-#pragma unroll
-                    for (int e = 8; e < kTile; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(sv[e]));
-                    const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-                    const float m_new = mx * p.scale_log2e;
-                    const bool grow = i == 0 || m_new > m_ref + 8.0f;
-                    float corr = 1.0f;
-                    if (grow) {
-                        const float m_tgt = fmaxf(m_ref, m_new);
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(corr) : "f"(m_ref - (m_tgt == -INFINITY ? 0.f : m_tgt)));
-                        m_ref = m_tgt;
-                    }
-                    // the S just waited for was committed behind this stream's last PV, so O is complete
-                    if (i > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t ov[32];
-                            tmem_ld32_nowait(o_addr + 32 * c, ov);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * corr);
-                            tmem_st32_nowait(o_addr + 32 * c, ov);
-                        }
-                        l *= corr;
-                    }
-                    // fp16 weights are stored as 2^(s - m_ref + 7): a key rounds to zero below 2^-32 of the reference only
-                    constexpr float kShift = BF16 ? 0.0f : 7.0f;
-                    const float neg_m = kShift - (m_ref == -INFINITY ? 0.f : m_ref);
-                    float ls0 = 0.f, ls1 = 0.f, ls2 = 0.f, ls3 = 0.f;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t packed[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            float p0, p1;
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(fmaf(__uint_as_float(sv[64 * c + 2 * e]), p.scale_log2e, neg_m)));
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(fmaf(__uint_as_float(sv[64 * c + 2 * e + 1]), p.scale_log2e, neg_m)));
-                            if (e & 1) { ls2 += p0; ls3 += p1; } else { ls0 += p0; ls1 += p1; }
-                            if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[e]) : "f"(p1), "f"(p0));
-                            else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(packed[e]) : "f"(p1), "f"(p0));
-                        }
-                        tmem_st32_nowait(s_addr + 32 * c, packed);
-                    }
-                    l += (ls0 + ls1) + (ls2 + ls3);
-                    tmem_wait_st();
-                }
-                // tokens of the tile that no row of the unit sees: their values are cleared (thread r owns token r); the two
-                // streams of a pair share the tile and stream 0, whose product reads it first, does it
-                if ((!pair || g == 0) && (t0 + kTile > kv_len || (t0 < lo_unit && t0 + kTile > sinks))) {
-                    const uint32_t place = base + (uint32_t)v_place(t, pair, it.count), slot = place % C::SLOTS;
-                    ptx::mbar_wait(&bars->full[slot], (place / C::SLOTS) & 1, abort_word);
+                // tokens of the tile that no row of the unit sees: their values are cleared (thread r owns token r).  The two
+                // streams of a pair share the tile; each clears it before its own product, and the second zero changes nothing
+                if (t0 + kTile > kv_len || (t0 < lo_unit && t0 + kTile > sinks)) {
+                    const uint32_t slot = 2 * (t % C::PLACES) + 1;
+                    ptx::mbar_wait(&bars->full[slot], uses.use_of(t) & 1, abort_word);
                     const int tok = t0 + r;
                     if (tok >= kv_len || (tok < lo_unit && tok >= sinks)) {
 #pragma unroll
@@ -441,10 +510,87 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     }
                     ptx::fence_proxy_async();  // the tensor core reads V through the async proxy
                 }
+                if (!dead) {
+                    if (!whole) mask_scores(s_addr, [&](int b) {
+                        uint64_t seen = key_range(lo, hi, b) | key_range(0, min(sinks, hi), b);
+                        if (tree && b + 64 > ctx && b < kv_len) {
+                            const int j = b - ctx;  // new token that key b is
+                            if (j >= 0) {
+                                seen |= tree_word(p.vis, bits, j >> 6, q_len) >> (j & 63);
+                                if (j & 63) seen |= tree_word(p.vis, bits, (j >> 6) + 1, q_len) << (64 - (j & 63));
+                            } else if (j > -64) {
+                                seen |= tree_word(p.vis, bits, 0, q_len) << (-j);
+                            }
+                        }
+                        return seen;
+                    }, t0);
+                    uint32_t sv[kTile];
+#pragma unroll
+                    for (int c = 0; c < kTile / 32; ++c) tmem_ld32_nowait(s_addr + 32 * c, sv + 32 * c);
+                    tmem_wait_ld();
+                    // The first half's weights are made with the reference the row has, and the tile's maximum is taken beside
+                    // them, in issue slots the special-function unit leaves; only when it has outgrown the reference (the
+                    // first tile, rarely a later one) are they made again.
+                    // fp16 weights are stored as 2^(s - m_ref + 7): a key rounds to zero below 2^-32 of the reference only
+                    constexpr float kShift = BF16 ? 0.0f : 7.0f;
+                    const uint64_t scale2 = pack2f(p.scale_log2e, p.scale_log2e);
+                    uint64_t sum2[2], neg2;
+                    auto weights = [&](int c) {  // 32 keys
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint64_t x = fma2(pack2u(sv[32 * c + 2 * e], sv[32 * c + 2 * e + 1]), scale2, neg2);
+                            uint64_t y;
+                            if (kPolyPeriod > 0 && e % kPolyPeriod == kPolyPeriod - 1) y = exp2_poly2(x);
+                            else y = pack2f(ex2(__uint_as_float((uint32_t)x)), ex2(__uint_as_float((uint32_t)(x >> 32))));
+                            sum2[e & 1] = add2(sum2[e & 1], y);
+                            const float p0 = __uint_as_float((uint32_t)y), p1 = __uint_as_float((uint32_t)(y >> 32));
+                            if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[e]) : "f"(p1), "f"(p0));
+                            else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(packed[e]) : "f"(p1), "f"(p0));
+                        }
+                        tmem_st16_nowait(s_addr + 16 * c, packed);
+                    };
+#pragma unroll 1
+                    for (;;) {
+                        const float neg_m = kShift - (m_ref == -INFINITY ? 0.f : m_ref);
+                        neg2 = pack2f(neg_m, neg_m);
+                        sum2[0] = sum2[1] = 0;
+                        weights(0);
+                        weights(1);
+                        float mx4[4];  // independent chains
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx4[e] = __uint_as_float(sv[e]);
+#pragma unroll
+                        for (int e = 4; e + 1 < kTile; e += 2) mx4[(e >> 1) & 3] = max3(mx4[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+                        const float m_new = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2e;
+                        const bool grow = m_new > m_ref + 8.0f || (m_ref == -INFINITY && m_new > m_ref);
+                        if (!__any_sync(0xffffffffu, grow)) break;
+                        // (the S waited for was committed behind this stream's last PV, so O is complete)
+                        float corr = 1.0f;
+                        if (grow) {
+                            corr = ex2(m_ref - m_new);
+                            m_ref = m_new;
+                        }
+                        if (i > 0) {
+                            scale_columns(o_addr, D / 32, corr);
+                            l *= corr;
+                        }
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    ptx::mbar_arrive(&bars->p_half[g]);
+                    weights(2);
+                    weights(3);
+                    const uint64_t both = add2(sum2[0], sum2[1]);
+                    l += __uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32));
+                    tmem_wait_st();
+                } else {
+                    ptx::mbar_arrive(&bars->p_half[g]);
+                }
                 tc_fence_before();
                 ptx::mbar_arrive(&bars->p_ready[g]);
             }
-            base += 2u * (uint32_t)it.count;
+            uses.finish(it.count);
 
             // ---------------------------------------------------------------- the item's rows
             const bool other_ran = pair || it.count > 1;
@@ -462,8 +608,8 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 const float m_o = xch[(2 * (g ^ 1)) * kRowBlock + r], l_o = xch[(2 * (g ^ 1) + 1) * kRowBlock + r];
                 exchange();
                 const float M = fmaxf(m_ref, m_o), M_safe = M == -INFINITY ? 0.f : M;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(mine) : "f"(m_ref - M_safe));
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(theirs) : "f"(m_o - M_safe));
+                mine = ex2(m_ref - M_safe);
+                theirs = ex2(m_o - M_safe);
                 // both add in the same order and get the same sum
                 l_tot = g == 0 ? fmaf(l, mine, l_o * theirs) : fmaf(l_o, theirs, l * mine);
                 m_ref = M;
@@ -486,10 +632,6 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 tc_fence_after();
                 if (!pair && g == 1) c_end = 0;  // stream 0 had the only tile
             }
-            // (both phases move on with the item, waited for here or not: the other stream's last product of an earlier item is
-            // complete when a later one of this stream is, so a wait is never two phases behind)
-            o_phase[0] += 1;
-            o_phase[1] += other_ran ? 1 : 0;
             const bool store = block0 + r < R && !dead;
             const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
             const int oi = (block0 + r) / p.G, ohh = (block0 + r) - oi * p.G;
@@ -532,6 +674,10 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     }
                 }
             }
+            // the other stream's phase is seen through as well, so that no wait falls two phases behind it
+            if (pair) ptx::mbar_wait(&bars->o_full[g ^ 1], o_phase[g ^ 1] & 1, abort_word);
+            o_phase[0] += 1;
+            o_phase[1] += other_ran ? 1 : 0;
             tc_fence_before();
             ptx::fence_proxy_async();  // the next item's Q arrives by TMA over the memory of the exchange
             ptx::mbar_arrive(&bars->item_done);
@@ -549,24 +695,43 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
 }
 
 // Units that were split along their keys: one warp per row joins the parts' states (in part order) and stores the row.
-// Bound by L2: every state is read once.
+// Bound by L2: every state is read once.  The work list comes from before the attention kernel, whose CTAs had all seen it
+// complete when they let this grid start, so a row's whereabouts are looked up ahead of the wait; behind it a row takes
+// two round trips, the parts' rows on their way together with their maxima and sums.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) wide_combine_kernel(const __grid_constant__ WideParams p) {
-    grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
     const int split = p.plan[p.L.queue + 3];
     const PlanLayout& PL = p.L.base;
     constexpr size_t kSlot = WdCfg<D>::SLOT_FLOATS;
-    constexpr int V = D / 32;
+    constexpr int V = D / 32, kDeep = 8;
     const int total = split * p.Hkv * kWideRows;
+    bool waited = false;
     for (int row = blockIdx.x * 8 + (threadIdx.x >> 5); row < total; row += gridDim.x * 8) {
         const int sr = row % kWideRows, rest = row / kWideRows, head = rest % p.Hkv, k = rest / p.Hkv;
         const int u = p.plan[p.L.split_unit + 3 * k], parts = p.plan[p.L.split_unit + 3 * k + 1];
         const int seq = p.plan[PL.unit_seq[3] + u], qs = p.qsl[seq], R = (p.qsl[seq + 1] - qs) * p.G;
         const int r = p.plan[PL.unit_row0[3] + u] + sr;
-        if (r >= R) continue;
         const float* base = p.slots + (size_t)(p.plan[p.L.split_unit + 3 * k + 2] + head * parts) * kSlot;
+        if (r >= R) continue;
+        if (!waited) grid_dep_wait();
+        waited = true;
+        float v[kDeep][V];
+        auto load = [&](int j0) {
+#pragma unroll
+            for (int q = 0; q < kDeep; ++q) {
+                const float* src = base + (size_t)min(j0 + q, parts - 1) * kSlot + (size_t)sr * D + V * lane;
+                if constexpr (V == 4) {
+                    const float4 x = __ldcg((const float4*)src);
+                    v[q][0] = x.x; v[q][1] = x.y; v[q][2] = x.z; v[q][3] = x.w;
+                } else {
+                    const float2 x = __ldcg((const float2*)src);
+                    v[q][0] = x.x; v[q][1] = x.y;
+                }
+            }
+        };
+        load(0);
         float M = -INFINITY;
         for (int j = lane; j < parts; j += 32)
             if (__ldcg(base + j * kSlot + kWideRows * (D + 1) + sr) > 0.f) M = fmaxf(M, __ldcg(base + j * kSlot + kWideRows * D + sr));
@@ -575,35 +740,21 @@ __global__ void __launch_bounds__(256) wide_combine_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = 0.f;
         for (int j0 = 0; j0 < parts; j0 += 32) {
-            const int jl = j0 + lane;
+            const int jl = j0 + lane, n = min(32, parts - j0);
             const float lp = jl < parts ? __ldcg(base + jl * kSlot + kWideRows * (D + 1) + sr) : 0.f;
             const float mp = jl < parts ? __ldcg(base + jl * kSlot + kWideRows * D + sr) : -INFINITY;
-            float w = 0.f;
-            if (lp > 0.f) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(mp - M));
+            const float w = lp > 0.f ? ex2(mp - M) : 0.f;
             den += warp_sum(w * lp);
-            const int n = min(32, parts - j0);
-            constexpr int kDeep = 8;
             for (int j = 0; j < n; j += kDeep) {
-                float v[kDeep][V], wj[kDeep];
+                if (j0 + j > 0) load(j0 + j);
 #pragma unroll
                 for (int q = 0; q < kDeep; ++q) {
-                    wj[q] = __shfl_sync(0xffffffffu, w, (j + q) & 31);
-                    if (j + q >= n) wj[q] = 0.f;
-                    const float* src = base + (size_t)(j0 + min(j + q, n - 1)) * kSlot + (size_t)sr * D + V * lane;
-                    if constexpr (V == 4) {
-                        const float4 x = __ldcg((const float4*)src);
-                        v[q][0] = x.x; v[q][1] = x.y; v[q][2] = x.z; v[q][3] = x.w;
-                    } else {
-                        const float2 x = __ldcg((const float2*)src);
-                        v[q][0] = x.x; v[q][1] = x.y;
+                    const float wj = __shfl_sync(0xffffffffu, w, (j + q) & 31);
+                    if (j + q < n && wj > 0.f) {  // a part in which the row sees nothing holds no numbers
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[e] = fmaf(wj, v[q][e], acc[e]);
                     }
                 }
-#pragma unroll
-                for (int q = 0; q < kDeep; ++q)
-                    if (wj[q] > 0.f) {  // a part in which the row sees nothing holds no numbers
-#pragma unroll
-                        for (int e = 0; e < V; ++e) acc[e] = fmaf(wj[q], v[q][e], acc[e]);
-                    }
             }
         }
         const float inv = den > 0.f ? 1.0f / den : 0.f;
@@ -617,6 +768,7 @@ __global__ void __launch_bounds__(256) wide_combine_kernel(const __grid_constant
             dst[e] = w;
         }
     }
+    if (!waited) grid_dep_wait();  // what follows in the stream relies on this grid for the one before it as well
 }
 
 // ------------------------------------------------------------------------------------------ host

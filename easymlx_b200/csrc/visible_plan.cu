@@ -11,6 +11,16 @@ __global__ void __launch_bounds__(kVpThreads) visible_plan_kernel(const VisibleP
     grid_dep_wait();
     grid_dep_launch();
     if (blockIdx.x == 0) {
+        __shared__ int32_t s_q[kVpSeqs + 1], s_kv[kVpSeqs];
+        if (S <= kVpSeqs) {
+            for (int s = threadIdx.x; s <= S; s += kVpThreads) {
+                s_q[s] = qsl[s];
+                if (s < S) s_kv[s] = kv_lens[s];
+            }
+            __syncthreads();
+            qsl = s_q;
+            kv_lens = s_kv;
+        }
         build_visible_plan(a, vis, qsl, kv_lens, S, scan_smem, status);
         return;
     }

@@ -20,6 +20,11 @@ constexpr int kVpThreads = 256;      // CTA width of everything that builds this
 constexpr int kWideRows = 256;       // rows of a class-3 unit
 constexpr int kMinSplitTiles = 4;    // a unit is never cut into parts shorter than this
 constexpr int kVpBins = kVpThreads;
+constexpr int kVpSeqs = 2048;        // offsets and tile prefixes up to these counts stay in shared memory: a search in global
+constexpr int kVpUnits = 2304;       // memory is a chain of L2 round trips, half a microsecond each
+constexpr int kMinSliceTiles = 2;    // a CTA of the short-row classes gets at least so many tiles: more parts than that only
+                                     // lengthen the join of a unit's states
+constexpr int kPlanAbsentShift = 16; // plan flag bits 16-19: row classes that the caller knows do not occur
 
 struct VisibleLayout {
     PlanLayout base;            // class 3: unit_seq, unit_row0, unit_tile_lo, unit_cum
@@ -59,7 +64,7 @@ __host__ __device__ inline VisibleLayout visible_layout(int S, int T, int Hq, in
 struct VisiblePlanArgs {
     int32_t* plan;
     VisibleLayout L;
-    int G, Hkv, num_ctas, class_lo, class_hi, wide, two_per_sm;
+    int G, Hkv, num_ctas, class_lo, class_hi, wide, two_per_sm, absent;
 };
 
 // Exclusive prefix of one value per thread over a CTA of THREADS threads; smem: THREADS / 32 + 1 words.
@@ -135,6 +140,7 @@ __device__ __forceinline__ void write_effective_mask(const Visibility& vis, int6
 __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, const Visibility& vis, const int32_t* qsl,
                                                    const int32_t* kv_lens, int S, int32_t* scan_smem, int32_t* status) {
     __shared__ int32_t bins[kVpBins];
+    __shared__ int32_t s_off[kVpSeqs], s_cum[kVpUnits + 1];
     __shared__ int s_chunk, s_max;
     const int tid = threadIdx.x;
     const PlanLayout& L = a.L.base;
@@ -145,7 +151,13 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
     }
     for (int c = 0; c < kNumClasses; ++c) {
         const int num_ctas = class_ctas(c, a.num_ctas, a.two_per_sm != 0);
-        if (c < a.class_lo || c > a.class_hi) {
+        bool mine = false;
+        if (c >= a.class_lo && c <= a.class_hi && !((a.absent >> c) & 1))
+            for (int s = tid; s < S; s += kVpThreads) {
+                const int q_len = qsl[s + 1] - qsl[s];
+                mine |= q_len > 0 && unit_class(q_len * a.G, a.wide != 0) == c;
+            }
+        if (!__syncthreads_or(mine)) {
             if (tid == 0) { plan[4 * c] = 0; plan[4 * c + 1] = 0; }
             if (c == 3) { if (tid < 4) plan[a.L.queue + tid] = 0; }
             else for (int i = tid; i <= num_ctas; i += kVpThreads) { plan[L.cta_start[c] + i] = 0; plan[L.cta_unit[c] + i] = 0; }
@@ -154,7 +166,7 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
         const int rows_c = c == 3 ? kWideRows : class_rows(c);
         int32_t *unit_seq = plan + L.unit_seq[c], *unit_row0 = plan + L.unit_row0[c];
         int32_t *unit_tile_lo = plan + L.unit_tile_lo[c], *unit_cum = plan + L.unit_cum[c];
-        int32_t* seq_off = plan + L.tmp;
+        int32_t* seq_off = S <= kVpSeqs ? s_off : plan + L.tmp;
         int num_units = 0;
         for (int s0 = 0; s0 < S; s0 += kVpThreads) {
             const int s = s0 + tid;
@@ -188,10 +200,15 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
             }
             int t_total;
             const int t_off = tile_base + scan_value<kVpThreads>(nt, scan_smem, t_total);
-            if (idx < num_units) unit_cum[idx] = t_off;
+            if (idx < num_units) {
+                unit_cum[idx] = t_off;
+                if (num_units <= kVpUnits) s_cum[idx] = t_off;
+            }
             tile_base += t_total;
         }
+        const int32_t* cum = num_units <= kVpUnits ? s_cum : unit_cum;
         if (tid == 0) {
+            if (num_units <= kVpUnits) s_cum[num_units] = tile_base;
             unit_cum[num_units] = tile_base;
             plan[4 * c] = num_units;
             plan[4 * c + 1] = tile_base;
@@ -200,7 +217,9 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
             for (int i = tid; i < num_units * a.Hkv; i += kVpThreads) plan[a.L.counters[c] + i] = 0;
         __syncthreads();
         if (c < 3) {
-            cut_slices<kVpThreads>(c, unit_cum, num_units, tile_base, a.Hkv, num_ctas, plan, L, num_ctas);
+            const long long tiles = (long long)tile_base * a.Hkv;
+            cut_slices<kVpThreads>(c, cum, num_units, tile_base, a.Hkv, num_ctas, plan, L,
+                                   (int)min((long long)num_ctas, (tiles + kMinSliceTiles - 1) / kMinSliceTiles));
             __syncthreads();
             continue;
         }
@@ -209,7 +228,7 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
         if (tid == 0) { s_chunk = 0x7fffffff; s_max = 1; }
         bins[tid] = 0;
         __syncthreads();
-        for (int u = tid; u < num_units; u += kVpThreads) atomicMax(&s_max, unit_cum[u + 1] - unit_cum[u]);
+        for (int u = tid; u < num_units; u += kVpThreads) atomicMax(&s_max, cum[u + 1] - cum[u]);
         __syncthreads();
         const long long total = (long long)tile_base * a.Hkv;
         const int share = max(kMinSplitTiles, (int)((total + a.num_ctas - 1) / a.num_ctas));
@@ -218,7 +237,7 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
             const int step = (longest - share + kVpThreads - 2) / (kVpThreads - 1);
             const int cand = share + tid * step;
             long long items = 0;
-            for (int u = 0; u < num_units; ++u) items += (unit_cum[u + 1] - unit_cum[u] + cand - 1) / cand;
+            for (int u = 0; u < num_units; ++u) items += (cum[u + 1] - cum[u] + cand - 1) / cand;
             if (items * a.Hkv <= a.num_ctas) atomicMin(&s_chunk, cand);
             __syncthreads();
         }
@@ -226,7 +245,7 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
         // entries: counting sort by decreasing length (longer ones than the last bin share it)
         auto parts_of = [&](int nt) { return (nt + chunk - 1) / chunk; };
         for (int u = tid; u < num_units; u += kVpThreads) {
-            const int nt = unit_cum[u + 1] - unit_cum[u], parts = parts_of(nt);
+            const int nt = cum[u + 1] - cum[u], parts = parts_of(nt);
             const int small = nt / parts, big = nt - small * parts;  // `big` parts of small + 1 tiles
             if (big) atomicAdd(&bins[kVpBins - 1 - min(small + 1, kVpBins - 1)], big);
             atomicAdd(&bins[kVpBins - 1 - min(small, kVpBins - 1)], parts - big);
@@ -241,7 +260,7 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
         for (int u0 = 0; u0 < num_units; u0 += kVpThreads) {
             const int u = u0 + tid;
             int nt = 0, parts = 0;
-            if (u < num_units) { nt = unit_cum[u + 1] - unit_cum[u]; parts = parts_of(nt); }
+            if (u < num_units) { nt = cum[u + 1] - cum[u]; parts = parts_of(nt); }
             int split_total, slot_total;
             const int split_idx = split_base + scan_value<kVpThreads>(parts > 1 ? 1 : 0, scan_smem, split_total);
             const int slot = slot_base + scan_value<kVpThreads>(parts > 1 ? parts * a.Hkv : 0, scan_smem, slot_total);
@@ -292,6 +311,7 @@ inline int visible_plan_args(VisiblePlanArgs* a, int S, int T, int Hq, int Hkv, 
     a->num_ctas = num_sms() < kMaxGrid ? num_sms() : kMaxGrid;
     a->wide = (plan_flags & kPlanWideUnits) != 0;
     a->two_per_sm = (plan_flags & kPlanTwoCtas) != 0;
+    a->absent = (plan_flags >> kPlanAbsentShift) & 15;
     class_range(a->G, max_query_len, a->wide != 0, a->class_lo, a->class_hi);
     return EMLX_OK;
 }

@@ -18,6 +18,17 @@ from .unified_attention import (_CHECK, _TILED_BLOCK_SIZE_AFFINE, _TILED_BLOCK_S
                                 _make_pool, _scratch, _validate_inputs)
 
 
+_status: dict = {}
+
+
+def _status_word(device) -> torch.Tensor:
+    """One word per device that every call ORs its faults into (a captured call must not bring a fill of its own)."""
+    word = _status.get(device)
+    if word is None:
+        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return word
+
+
 class VisibleAttentionCall:
     """One validated call, split like ``AttentionCall`` into ``plan()`` (work list) and ``launch()``.
 
@@ -28,7 +39,7 @@ class VisibleAttentionCall:
                  softmax_scale: float | None = None, sliding_window: int | None = None, sink_tokens: int = 0, tree_mask=None,
                  tree_seqs=None, k_scale=None, v_scale=None, k_bias=None, v_bias=None, kernel: str | None = None,
                  max_query_len: int = 0, plan=None, query_len_set: tp.Sequence[int] | None = None, long_seqs: int = 0):
-        from ...caching.paged.cache import VisiblePlan, native_visibility, tree_arguments, visible_plan_flags
+        from ...caching.paged.cache import VisiblePlan, absent_row_classes, native_visibility, tree_arguments, visible_plan_flags
 
         nv.require_cuda(queries, key_cache, value_cache)
         dev = queries.device
@@ -77,7 +88,7 @@ class VisibleAttentionCall:
                 "the same dtype (or an affine pool)")
         self.kernel = kernel or ("tiled" if tiled_ok else "generic")
         self.visibility = native_visibility(self.sinks, self.tree_mask, self.tree_seqs)
-        self.status = _scratch.get(dev, "status", 4, zero=True)
+        self.status = _status_word(dev)
         a = nv.AttnArgs()
         a.queries = self.queries.data_ptr()
         a.block_tables, a.kv_lens = self.block_tables.data_ptr(), self.kv_lens.data_ptr()
@@ -95,17 +106,14 @@ class VisibleAttentionCall:
         words = 0 if self.tree_mask is None else int(self.tree_mask.shape[1])
         flags = visible_plan_flags(self.pool.kv_format, self.hq, hkv, self.d, int(long_seqs))
         self.plan_bytes = int(lib.emlx_visible_plan_bytes(self.num_seqs, self.total, self.hq, hkv, words))
+        if query_len_set:
+            flags |= absent_row_classes(query_len_set, self.hq // hkv, bool(flags & 1))
         self.planned = (isinstance(plan, VisiblePlan) and plan.num_q_heads == self.hq and plan.sliding_window == self.window
                         and plan.sink_tokens == self.sinks and plan.flags == flags and plan.buffer.numel() >= self.plan_bytes
                         and plan.tree_mask is self.tree_mask and plan.tree_seqs is self.tree_seqs)
         self.plan_buf = plan.buffer if self.planned else torch.empty(self.plan_bytes, dtype=torch.uint8, device=dev)
         a.plan_flags = flags
-        if query_len_set:
-            group, wide = self.hq // hkv, bool(flags & 1)
-            for q_len in query_len_set:
-                rows = int(q_len) * group
-                if rows > 0:
-                    a.row_class_mask |= 1 << (0 if rows <= 8 else 1 if rows <= 16 else (3 if wide else 2))
+        a.row_class_mask = ~(flags >> 16) & 15 if flags >> 16 else 0
         ws_bytes = int(lib.emlx_visible_workspace_bytes(self.hq, hkv, self.d, int(a.max_query_len), flags))
         if affine and flags & 1:
             ws_bytes += int(lib.emlx_attn_dequant_bytes(self.pool, self.num_seqs, int(self.block_tables.shape[1]), int(long_seqs),

@@ -150,12 +150,12 @@ def test_calls_are_refused_on_the_host(lib):
     assert lib.emlx_positioned_write(None, None, 0, None, None, 0, 4, None, None, None, 0, None, None, None, None, None, None) == inv
 
     layers = (_native.CommitLayer * 1)()
-    assert lib.emlx_commit_tree(layers, 1, _pool(), 8, 1, 8, 2, 1, 1, 8, 8, None, None) == inv  # a layer without pointers
+    assert lib.emlx_commit_tree(ctypes.addressof(layers), 1, _pool(), 8, 1, 8, 2, 1, 1, 8, 8, None, None) == inv  # a layer without pointers
     layers[0].key_cache = layers[0].value_cache = layers[0].block_tables = layers[0].kv_lens = 4096
     layers[0].num_blocks = 4
-    assert lib.emlx_commit_tree(layers, 0, _pool(), 8, 1, 8, 2, 1, 1, 8, 8, None, None) == inv
-    assert lib.emlx_commit_tree(layers, 1, _pool(), None, 1, 8, 2, 1, 1, 8, 8, None, None) == inv
-    assert lib.emlx_commit_tree(layers, 1, _pool(), None, 0, None, 0, 1, 1, None, None, None, None) == _native.EMLX_OK
+    assert lib.emlx_commit_tree(ctypes.addressof(layers), 0, _pool(), 8, 1, 8, 2, 1, 1, 8, 8, None, None) == inv
+    assert lib.emlx_commit_tree(ctypes.addressof(layers), 1, _pool(), None, 1, 8, 2, 1, 1, 8, 8, None, None) == inv
+    assert lib.emlx_commit_tree(ctypes.addressof(layers), 1, _pool(), None, 0, None, 0, 1, 1, None, None, None, None) == _native.EMLX_OK
 
 
 def test_cpu_tensors_are_refused():
