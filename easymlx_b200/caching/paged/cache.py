@@ -860,7 +860,9 @@ def commit_layers(views: tp.Sequence[PageCacheView], slot_ids, accepted, *, adva
     if isinstance(slot_ids, torch.Tensor):
         if slot_ids.ndim != 1 or slot_ids.dtype.is_floating_point:
             raise ValueError("slot_ids must be rank-1 integers")
-        slots = slot_ids.to(device=dev, dtype=torch.int32).contiguous()
+        slots = slot_ids
+        if slots.dtype != torch.int32 or slots.device != dev or not slots.is_contiguous():
+            slots = slots.to(device=dev, dtype=torch.int32).contiguous()
     else:
         host = tuple(int(x) for x in slot_ids)
         if len(set(host)) != len(host):
@@ -879,14 +881,16 @@ def commit_layers(views: tp.Sequence[PageCacheView], slot_ids, accepted, *, adva
         raise ValueError(f"accepted must be integers [{s}, max_path], ended by -1")
     if accepted.is_cuda and accepted.device != dev:
         raise ValueError("accepted must be on the device of the cache")
-    accepted = accepted.to(device=dev, dtype=torch.int32).contiguous()
+    if accepted.dtype != torch.int32 or accepted.device != dev or not accepted.is_contiguous():
+        accepted = accepted.to(device=dev, dtype=torch.int32).contiguous()
     committed = torch.empty(s, dtype=torch.int32, device=dev)
     if s == 0:
         return committed
     with nv.on_device(dev):
-        nv.check(nv.lib().emlx_commit_tree(layers, len(views), rows[0][2], nv.ptr(slots), s, nv.ptr(accepted),
-                                           int(accepted.shape[1]), first.num_seqs, first.blocks_per_seq, nv.ptr(committed),
-                                           nv.ptr(first.ticket), nv.ptr(first.status), nv.stream_ptr(dev)))
+        nv.check(nv.lib().emlx_commit_tree(
+            layers, len(views), rows[0][2], slots.data_ptr(), s, accepted.data_ptr(), int(accepted.shape[1]), geometry[5],
+            geometry[6], committed.data_ptr(), first.ticket.data_ptr(), first.status.data_ptr(),
+            torch.cuda.current_stream(dev).cuda_stream))
     if _CHECK and not torch.cuda.is_current_stream_capturing():
         first.check()
     return committed

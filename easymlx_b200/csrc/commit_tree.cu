@@ -28,7 +28,7 @@ struct CommitParams {
     int32_t* committed;
     int32_t* ticket;
     int32_t* status;
-    int S, M, num_slots, MB, bs, Hkv, D, format, row_bytes, write_lens;
+    int S, M, num_slots, MB, bs, Hkv, D, format, row_bytes, write_lens, any_advance;
 };
 
 // `unit` bytes per thread and step; rows are `bytes` long and start at base + row * bytes.
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kCommitThreads) commit_tree_kernel(const __gri
             __syncthreads();
         }
     }
+    if (!p.any_advance) return;
     // every CTA of the launch has read the lengths when the last ticket is drawn
     __syncthreads();
     if (tid == 0) {
@@ -204,6 +205,8 @@ extern "C" int emlx_commit_tree(const emlx_commit_layer* layers, int32_t num_lay
             p.layer[y].advance = wanted && last;
         }
         p.write_lens = y0 == 0;
+        p.any_advance = 0;
+        for (int y = 0; y < n; ++y) p.any_advance |= p.layer[y].advance;
         EMLX_CUDA_OK(launch_pdl(commit_tree_kernel, dim3((unsigned)num_seqs, (unsigned)n), kCommitThreads, 0, (cudaStream_t)stream, p));
         EMLX_LAUNCHED();
     }

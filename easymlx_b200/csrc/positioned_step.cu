@@ -448,7 +448,8 @@ extern "C" int emlx_positioned_step(const emlx_step_args* a, const emlx_pool* po
         if (int rc = visible_plan_args(&p.plan, a->num_seqs, a->total_tokens, a->num_q_heads, pool->num_kv_heads, pool->block_size,
                                        a->query_lens ? a->max_query_len : 1, a->plan_flags, p.vis, a->plan, a->plan_bytes))
             return rc;
-    const unsigned grid = 1u + row_ctas(p, 3);
+    // every CTA scans the query lengths: with many sequences fewer CTAs loop, with few the scheduler deals out single groups
+    const unsigned grid = 1u + row_ctas(p, p.S <= kPosThreads ? 16 : 3);
     cudaStream_t s = (cudaStream_t)stream;
     switch (a->in_dtype) {
         case EMLX_F16: EMLX_CUDA_OK(launch_pdl(positioned_step_kernel<__half>, grid, kPosThreads, 0, s, p)); break;

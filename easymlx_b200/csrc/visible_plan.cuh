@@ -242,10 +242,21 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
             __syncthreads();
         }
         const int chunk = s_chunk == 0x7fffffff ? share : s_chunk;
+        // Units of about one length that fill some rounds of CTAs and then a part of one: the units of that last round are
+        // split over all CTAs.  (Units of mixed lengths fill the last round by themselves, the shortest come last.)
+        const int items = num_units * a.Hkv, last = items % a.num_ctas;
+        int tail_from = num_units, tail_parts = 1;
+        if (items > a.num_ctas && last > 0 && 2 * last <= a.num_ctas && (long long)longest * num_units * 4 <= (long long)tile_base * 5) {
+            tail_from = num_units - (last + a.Hkv - 1) / a.Hkv;
+            tail_parts = max(1, min(a.num_ctas / last, longest / kMinSplitTiles));
+        }
         // entries: counting sort by decreasing length (longer ones than the last bin share it)
-        auto parts_of = [&](int nt) { return (nt + chunk - 1) / chunk; };
+        auto parts_of = [&](int u) {
+            const int nt = cum[u + 1] - cum[u];
+            return u >= tail_from ? min(tail_parts, nt) : (nt + chunk - 1) / chunk;
+        };
         for (int u = tid; u < num_units; u += kVpThreads) {
-            const int nt = cum[u + 1] - cum[u], parts = parts_of(nt);
+            const int nt = cum[u + 1] - cum[u], parts = parts_of(u);
             const int small = nt / parts, big = nt - small * parts;  // `big` parts of small + 1 tiles
             if (big) atomicAdd(&bins[kVpBins - 1 - min(small + 1, kVpBins - 1)], big);
             atomicAdd(&bins[kVpBins - 1 - min(small, kVpBins - 1)], parts - big);
@@ -260,7 +271,7 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
         for (int u0 = 0; u0 < num_units; u0 += kVpThreads) {
             const int u = u0 + tid;
             int nt = 0, parts = 0;
-            if (u < num_units) { nt = cum[u + 1] - cum[u]; parts = parts_of(nt); }
+            if (u < num_units) { nt = cum[u + 1] - cum[u]; parts = parts_of(u); }
             int split_total, slot_total;
             const int split_idx = split_base + scan_value<kVpThreads>(parts > 1 ? 1 : 0, scan_smem, split_total);
             const int slot = slot_base + scan_value<kVpThreads>(parts > 1 ? parts * a.Hkv : 0, scan_smem, slot_total);
