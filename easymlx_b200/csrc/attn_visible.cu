@@ -67,7 +67,7 @@ int run_visible(const emlx_attn_args* a, const emlx_pool* pool, const emlx_visib
     if (pool->kv_format == EMLX_KV_FLOAT && pool->kv_dtype != a->q_dtype)
         return fail(EMLX_ERR_UNSUPPORTED, "the tiled kernels need the pool dtype to equal the query dtype");
     if (((uintptr_t)a->queries | (uintptr_t)a->out) & 15) return fail(EMLX_ERR_INVALID, "queries/out must be 16-byte aligned");
-    if ((uintptr_t)a->plan & 7) return fail(EMLX_ERR_INVALID, "plan must be 8-byte aligned");
+    if ((uintptr_t)a->plan & 15) return fail(EMLX_ERR_INVALID, "plan must be 16-byte aligned");
     if ((uintptr_t)a->workspace & 15) return fail(EMLX_ERR_INVALID, "workspace must be 16-byte aligned");
     const Visibility vis = make_visibility(visibility, a->sliding_window);
     const int words = vis.tree ? vis.words : 0;

@@ -84,20 +84,15 @@ struct WdBarriers {
 };
 static_assert(sizeof(WdBarriers) <= 512, "the barrier block has 512 bytes of shared memory");
 
-struct WideItem {
-    int u, head, j0, count, part, parts, slot;
+struct WideItem : WideEntry {
+    int head;
 };
 __device__ __forceinline__ WideItem wide_item(const WideParams& p, int idx) {
     WideItem it;
     const int e = idx / p.Hkv;
+    (WideEntry&)it = ((const WideEntry*)(p.plan + p.L.entry))[e];
     it.head = idx - e * p.Hkv;
-    it.u = p.plan[p.L.entry_unit + e];
-    it.j0 = p.plan[p.L.entry_tile + e];
-    it.count = p.plan[p.L.entry_count + e];
-    const int pp = p.plan[p.L.entry_part + e];
-    it.part = pp & 0xffff;
-    it.parts = pp >> 16;
-    it.slot = p.plan[p.L.entry_slot + e] + it.head * it.parts;
+    it.slot += it.head * it.parts;
     return it;
 }
 // Uses of the ring's places so far: every role counts them the same way, item by item.
@@ -245,8 +240,6 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     grid_dep_launch();
     int32_t* queue = p.plan + p.L.queue;
     const int items = p.plan[p.L.queue + 2] * p.Hkv;
-    const PlanLayout& PL = p.L.base;
-    const int32_t *unit_seq = p.plan + PL.unit_seq[3], *unit_row0 = p.plan + PL.unit_row0[3], *unit_tile_lo = p.plan + PL.unit_tile_lo[3];
 
     if (warp >= kWdProducer) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWdOtherRegs));
@@ -267,11 +260,10 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 if (idx < 0) break;
                 if (lane == 0) next = atomicAdd(queue, 1);  // the following item, drawn while this one is loaded
                 const WideItem it = wide_item(p, idx);
-                const int seq = unit_seq[it.u], row0 = unit_row0[it.u], tile_lo = unit_tile_lo[it.u];
-                const int qs = p.qsl[seq], q_len = p.qsl[seq + 1] - qs, kv_len = p.kv_lens[seq];
+                const int seq = it.seq, row0 = it.row0, tile_lo = it.tile_lo, qs = it.qs, q_len = it.q_len, kv_len = it.kv_len;
                 const bool pair = q_len * p.G - row0 > kRowBlock;
                 const int sinks_in = sink_tiles(p.vis.sinks, tile_lo);
-                const int lo = unit_lo(p.vis, is_tree(p.vis, seq), row0, p.G, kv_len - q_len, kv_len);
+                const int lo = unit_lo(p.vis, it.tree != 0, row0, p.G, kv_len - q_len, kv_len);
                 // The item's Q replaces the last one's: every QK of that item must have read it, and where its streams joined
                 // their states through the same memory, its rows must be stored.  (The done phases are waited for in turn, so
                 // that none is two phases behind.)
@@ -359,8 +351,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 const int idx = bars->item_ring[k & 3];
                 if (idx < 0) break;
                 const WideItem it = wide_item(p, idx);
-                const int seq = unit_seq[it.u], row0 = unit_row0[it.u];
-                const bool pair = (p.qsl[seq + 1] - p.qsl[seq]) * p.G - row0 > kRowBlock;
+                const bool pair = it.q_len * p.G - it.row0 > kRowBlock;
                 const int steps = pair ? it.count : (it.count - s + 1) / 2, other = pair ? it.count : (it.count - (s ^ 1) + 1) / 2;
                 ptx::mbar_wait(&bars->q_full, k & 1, abort_word);
                 if (steps == 0 && lane == 0) ptx::mbar_arrive(&bars->q_free);
@@ -444,10 +435,9 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             const int idx = bars->item_ring[k & 3];
             if (idx < 0) break;
             const WideItem it = wide_item(p, idx);
-            const int seq = unit_seq[it.u], row0 = unit_row0[it.u], tile_lo = unit_tile_lo[it.u];
-            const int qs = p.qsl[seq], q_len = p.qsl[seq + 1] - qs, kv_len = p.kv_lens[seq];
+            const int row0 = it.row0, tile_lo = it.tile_lo, qs = it.qs, q_len = it.q_len, kv_len = it.kv_len;
             const int R = q_len * p.G, ctx = kv_len - q_len;
-            const bool pair = R - row0 > kRowBlock, tree = is_tree(p.vis, seq);
+            const bool pair = R - row0 > kRowBlock, tree = it.tree != 0;
             const int sinks_in = sink_tiles(p.vis.sinks, tile_lo);
             const int block0 = row0 + (pair ? kRowBlock * g : 0);     // first row of this stream
             const int rows_here = min(kRowBlock, R - block0);
@@ -682,18 +672,16 @@ __global__ void __launch_bounds__(256, 4) wide_combine_kernel(const __grid_const
     grid_dep_launch();
     const int lane = threadIdx.x & 31;
     const int split = p.plan[p.L.queue + 3];
-    const PlanLayout& PL = p.L.base;
     constexpr size_t kSlot = WdCfg<D>::SLOT_FLOATS;
     constexpr int V = D / 32, kDeep = 8;
     const int total = split * p.Hkv * kWideRows;
     bool waited = false;
     for (int row = blockIdx.x * 8 + (threadIdx.x >> 5); row < total; row += gridDim.x * 8) {
         const int sr = row % kWideRows, rest = row / kWideRows, head = rest % p.Hkv, k = rest / p.Hkv;
-        const int u = p.plan[p.L.split_unit + 3 * k], parts = p.plan[p.L.split_unit + 3 * k + 1];
-        const int seq = p.plan[PL.unit_seq[3] + u], qs = p.qsl[seq], R = (p.qsl[seq + 1] - qs) * p.G;
-        const int r = p.plan[PL.unit_row0[3] + u] + sr;
-        const float* base = p.slots + (size_t)(p.plan[p.L.split_unit + 3 * k + 2] + head * parts) * kSlot;
-        if (r >= R) continue;
+        const WideSplit sp = ((const WideSplit*)(p.plan + p.L.split))[k];
+        if (sr >= sp.rows) continue;
+        const int parts = sp.parts, qs = sp.qs, r = sp.row0 + sr;
+        const float* base = p.slots + (size_t)(sp.slot + head * parts) * kSlot;
         if (!waited) grid_dep_wait();
         waited = true;
         float v[kDeep][V];

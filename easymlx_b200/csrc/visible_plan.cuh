@@ -26,16 +26,24 @@ constexpr int kMinSliceTiles = 2;    // a CTA of the short-row classes gets at l
                                      // lengthen the join of a unit's states
 constexpr int kPlanAbsentShift = 16; // plan flag bits 16-19: row classes that the caller knows do not occur
 
+// All that an item needs to know, so that it starts with one round of loads instead of a chain entry -> unit -> sequence.
+struct alignas(16) WideEntry {
+    int j0, count;              // first tile (index inside the unit) and tiles
+    int part, parts;
+    int slot;                   // partial slot of head 0; slot of head h: + h * parts
+    int seq, row0, tile_lo;
+    int qs, q_len, kv_len, tree;
+};
+struct alignas(16) WideSplit {
+    int parts, slot, row0, rows, qs, pad[3];
+};
+
 struct VisibleLayout {
     PlanLayout base;            // class 3: unit_seq, unit_row0, unit_tile_lo, unit_cum
     int counters[3];            // arrival counters of the short-row classes, cap * Hkv words each
     int queue;                  // class 3: [0] next item, [1] CTAs done, [2] entries, [3] split units
-    int entry_unit;             // class 3 entries, longest first
-    int entry_tile;             // first tile (index inside the unit)
-    int entry_count;
-    int entry_part;             // part | parts << 16
-    int entry_slot;             // partial slot of (head 0, this part); slot of head h: + h * parts
-    int split_unit;             // units that were split: unit, parts, first slot
+    int entry;                  // class 3: WideEntry records, longest first (16-byte aligned)
+    int split;                  // WideSplit records of the units that were split
     int max_entries, max_split;
     int eff;                    // windowed masks, T * words 64-bit words (8-byte aligned), only under a window
     int words;                  // 32-bit words in all
@@ -49,12 +57,9 @@ __host__ __device__ inline VisibleLayout visible_layout(int S, int T, int Hq, in
     V.queue = w; w += 8;
     V.max_split = 2 * kMaxGrid;
     V.max_entries = V.base.cap[3] + V.max_split;
-    V.entry_unit = w; w += V.max_entries;
-    V.entry_tile = w; w += V.max_entries;
-    V.entry_count = w; w += V.max_entries;
-    V.entry_part = w; w += V.max_entries;
-    V.entry_slot = w; w += V.max_entries;
-    V.split_unit = w; w += 3 * V.max_split;
+    w = (w + 3) & ~3;
+    V.entry = w; w += V.max_entries * (int)(sizeof(WideEntry) / 4);
+    V.split = w; w += V.max_split * (int)(sizeof(WideSplit) / 4);
     w = (w + 1) & ~1;
     V.eff = w; w += 2 * T * tree_words;
     V.words = w;
@@ -275,20 +280,23 @@ __device__ __forceinline__ void build_visible_plan(const VisiblePlanArgs& a, con
             int split_total, slot_total;
             const int split_idx = split_base + scan_value<kVpThreads>(parts > 1 ? 1 : 0, scan_smem, split_total);
             const int slot = slot_base + scan_value<kVpThreads>(parts > 1 ? parts * a.Hkv : 0, scan_smem, slot_total);
+            WideEntry rec{};
+            if (parts > 0) {
+                rec.parts = parts; rec.seq = unit_seq[u]; rec.row0 = unit_row0[u]; rec.tile_lo = unit_tile_lo[u];
+                rec.qs = qsl[rec.seq]; rec.q_len = qsl[rec.seq + 1] - rec.qs; rec.kv_len = kv_lens[rec.seq];
+                rec.tree = is_tree(vis, rec.seq) ? 1 : 0;
+            }
             if (parts > 1) {
-                plan[a.L.split_unit + 3 * split_idx] = u;
-                plan[a.L.split_unit + 3 * split_idx + 1] = parts;
-                plan[a.L.split_unit + 3 * split_idx + 2] = slot;
+                WideSplit sp{};
+                sp.parts = parts; sp.slot = slot; sp.row0 = rec.row0; sp.rows = min(kWideRows, rec.q_len * a.G - rec.row0); sp.qs = rec.qs;
+                ((WideSplit*)(plan + a.L.split))[split_idx] = sp;
             }
             const int small = parts ? nt / parts : 0, big = nt - small * parts;
             for (int k = 0, at = 0; k < parts; ++k) {
                 const int count = small + (k < big ? 1 : 0);
                 const int e = atomicAdd(&bins[kVpBins - 1 - min(count, kVpBins - 1)], 1);
-                plan[a.L.entry_unit + e] = u;
-                plan[a.L.entry_tile + e] = at;
-                plan[a.L.entry_count + e] = count;
-                plan[a.L.entry_part + e] = k | (parts << 16);
-                plan[a.L.entry_slot + e] = slot + k;
+                rec.j0 = at; rec.count = count; rec.part = k; rec.slot = slot + k;
+                ((WideEntry*)(plan + a.L.entry))[e] = rec;
                 at += count;
             }
             split_base += split_total;
@@ -315,7 +323,7 @@ inline int visible_plan_args(VisiblePlanArgs* a, int S, int T, int Hq, int Hkv, 
     const int words = vis.tree ? vis.words : 0;
     if (!plan || plan_bytes < visible_plan_bytes(S, T, Hq, Hkv, words))
         return fail(EMLX_ERR_WORKSPACE, "plan buffer missing or smaller than emlx_visible_plan_bytes()");
-    if ((uintptr_t)plan & 7) return fail(EMLX_ERR_INVALID, "plan must be 8-byte aligned");
+    if ((uintptr_t)plan & 15) return fail(EMLX_ERR_INVALID, "plan must be 16-byte aligned");
     a->plan = (int32_t*)plan;
     a->L = visible_layout(S, T, Hq, Hkv, words);
     a->G = Hq / Hkv; a->Hkv = Hkv;

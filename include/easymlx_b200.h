@@ -310,7 +310,7 @@ int emlx_attn_visible_generic(const emlx_attn_args* args, const emlx_pool* pool,
 
 /* Work list of an attention call over these rows (built by emlx_positioned_step as well).  plan_flags as for
  * emlx_attn_plan; bits 16-19 may name row classes (emlx_attn_row_class) that do not occur in the batch.  It also holds the call's
- * counters: calls that may overlap on the GPU need lists of their own.  8-byte aligned; tree_words = 0 without a mask. */
+ * counters: calls that may overlap on the GPU need lists of their own.  16-byte aligned; tree_words = 0 without a mask. */
 size_t emlx_visible_plan_bytes(int32_t num_seqs, int32_t total_tokens, int32_t num_q_heads, int32_t num_kv_heads,
                                int32_t tree_words);
 int emlx_visible_plan(const int32_t* query_start_loc, const int32_t* kv_lens, int32_t num_seqs, int32_t total_tokens,

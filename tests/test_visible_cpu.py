@@ -124,10 +124,10 @@ def test_calls_are_refused_on_the_host(lib):
     assert lib.emlx_attn_visible_generic(args, _pool(head_dim=512), vis, None) == uns
     n = lib.emlx_visible_plan_bytes(4, 64, 8, 2, 1)
     assert n > lib.emlx_attn_plan_bytes(4, 64, 8, 2) and lib.emlx_visible_plan_bytes(4, 64, 8, 0, 1) == 0
-    assert lib.emlx_visible_plan(8, 8, 4, 64, 8, 2, 128, 0, vis, 0, 0, 8, n - 1, None, None) == work
-    assert lib.emlx_visible_plan(8, 8, 4, 64, 8, 2, 48, 0, vis, 0, 0, 8, n, None, None) == uns
-    assert lib.emlx_visible_plan(8, 8, 4, 64, 7, 2, 128, 0, vis, 0, 0, 8, n, None, None) == inv
-    assert lib.emlx_visible_plan(8, 8, 4, 64, 8, 2, 128, 0, vis, 0, 0, 4, n, None, None) == inv  # misaligned
+    assert lib.emlx_visible_plan(8, 8, 4, 64, 8, 2, 128, 0, vis, 0, 0, 16, n - 1, None, None) == work
+    assert lib.emlx_visible_plan(8, 8, 4, 64, 8, 2, 48, 0, vis, 0, 0, 16, n, None, None) == uns
+    assert lib.emlx_visible_plan(8, 8, 4, 64, 7, 2, 128, 0, vis, 0, 0, 16, n, None, None) == inv
+    assert lib.emlx_visible_plan(8, 8, 4, 64, 8, 2, 128, 0, vis, 0, 0, 8, n, None, None) == inv  # misaligned
 
     step = _native.StepArgs()
     assert lib.emlx_positioned_step(step, _pool(), None, None, None, None) == _native.EMLX_OK  # no sequences
