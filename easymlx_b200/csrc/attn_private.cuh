@@ -17,7 +17,7 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
 constexpr int kHelpParts = 128;  // longest list of parts the job area holds
 constexpr int kHelpMinParts = 6; // below this the one-warp fold is as fast
 constexpr int kMiscHelpExit = 8; // misc[]: the merge warp has left, parked warps may go
-template <int D, int NT, int FMT, bool BF16, bool PEER>
+template <int D, int NT, int FMT, bool BF16, bool PEER, bool VIS>
 __device__ __forceinline__ void park_consumer_warp(const TiledParams& p, uint8_t* fixed, uint64_t* full,
                                                    volatile int* abort_word);
 template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -340,6 +340,16 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
                         ptx::fence_proxy_async();
                         __syncwarp();
                     }
+                    if constexpr (VIS) {
+                        if (q_len > 1) {
+                            const uint32_t odd = take_out_odd_values<D, BF16>(st + C::KBYTES, 16 * warp, lane);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    if (((odd >> (c < 2 ? g : g + 8)) & 1) && s[nt][c] != -INFINITY) l[nt][c & 1] = __int_as_float(0x7fffffff);
+                        }
+                    }
                 }
             }
 
@@ -529,7 +539,7 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
                 if (complete) {
                     const int r = row0 + row;
                     if (r < R) {
-                        const float inv = L > 0.f ? 1.0f / L : 0.f;
+                        const float inv = holds<VIS>(L) ? 1.0f / L : 0.f;
                         const int i = r / p.G, hh = r - i * p.G;
                         uint2 packed;
                         packed.x = pack2<BF16>(acc.x * inv, acc.y * inv);
@@ -583,7 +593,7 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
         if (lane == 0) ptx::mbar_arrive(&mfull[posted]);
     }
     if constexpr (HELP) {
-        if (may_help) park_consumer_warp<D, NT, FMT, BF16, PEER>(p, fixed, full, abort_word);
+        if (may_help) park_consumer_warp<D, NT, FMT, BF16, PEER, VIS>(p, fixed, full, abort_word);
     }
 }
 
@@ -605,7 +615,7 @@ struct MergeJob {
     float l[kHelpParts][ROWS];            // sum of part j for row r
 };
 
-template <int D, int NT, int FMT, bool BF16, bool PEER>
+template <int D, int NT, int FMT, bool BF16, bool PEER, bool VIS>
 __device__ __forceinline__ void help_merge(const TiledParams& p, const MergeJob<Cfg<D, NT, FMT>::ROWS>* job, int warp, int lane) {
     constexpr int ROWS = Cfg<D, NT, FMT>::ROWS, V = D / 32, B = 8;
     const int nparts = job->nparts;
@@ -643,7 +653,7 @@ __device__ __forceinline__ void help_merge(const TiledParams& p, const MergeJob<
         const long long dst = out_offset<D>(p, rq.qs + i, rq.head * p.G + hh) + V * lane;
         float o[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = dr > 0.f ? acc[k] / dr : 0.f;
+        for (int k = 0; k < V; ++k) o[k] = holds<VIS>(dr) ? acc[k] / dr : 0.f;
         if constexpr (V == 4) {
             uint2 packed;
             packed.x = pack2<BF16>(o[0], o[1]);
@@ -660,7 +670,7 @@ __device__ __forceinline__ void help_merge(const TiledParams& p, const MergeJob<
 }
 
 // Consumer warps that have finished their slice: wait for jobs of the merge warp until it says that it has left.
-template <int D, int NT, int FMT, bool BF16, bool PEER>
+template <int D, int NT, int FMT, bool BF16, bool PEER, bool VIS>
 __device__ __forceinline__ void park_consumer_warp(const TiledParams& p, uint8_t* fixed, uint64_t* full,
                                                    volatile int* abort_word) {
     using C = Cfg<D, NT, FMT>;
@@ -684,7 +694,7 @@ __device__ __forceinline__ void park_consumer_warp(const TiledParams& p, uint8_t
             return;
         }
         if (misc[kMiscHelpExit]) return;
-        help_merge<D, NT, FMT, BF16, PEER>(p, (const MergeJob<C::ROWS>*)(fixed + C::PBYTES), warp, lane);
+        help_merge<D, NT, FMT, BF16, PEER, VIS>(p, (const MergeJob<C::ROWS>*)(fixed + C::PBYTES), warp, lane);
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(done);
     }
@@ -693,7 +703,7 @@ __device__ __forceinline__ void park_consumer_warp(const TiledParams& p, uint8_t
 // The merge warp.  For every unfinished part the consumers hand over: make the slot visible to the GPU, count the
 // arrival on the (unit, head) counter, and when this was the last of the unit's parts, fold all of them in slice
 // order (so the result does not depend on which CTA came last) and write the rows.
-template <int D, int NT, int FMT, bool BF16, bool PEER, bool HELP>
+template <int D, int NT, int FMT, bool BF16, bool PEER, bool HELP, bool VIS>
 __device__ __forceinline__ void merge_warp_loop(const TiledParams& p, uint8_t* fixed, uint64_t* full,
                                                 volatile int* abort_word, int active) {
     using C = Cfg<D, NT, FMT>;
@@ -770,7 +780,7 @@ __device__ __forceinline__ void merge_warp_loop(const TiledParams& p, uint8_t* f
                 }
 #pragma unroll
                 for (int row = 0; row < ROWS; ++row) {
-                    Mr[row] = fmaxf(Mr[row], warp_max(lp[row] > 0.f ? mp[row] : -INFINITY));
+                    Mr[row] = fmaxf(Mr[row], warp_max(holds<VIS>(lp[row]) ? mp[row] : -INFINITY));
                     if (c <= c_last) {
                         job->w[base + lane][row] = mp[row];  // the maximum for now; the weight once M is known
                         job->l[base + lane][row] = lp[row];
@@ -782,7 +792,7 @@ __device__ __forceinline__ void merge_warp_loop(const TiledParams& p, uint8_t* f
 #pragma unroll
                 for (int row = 0; row < ROWS; ++row) {
                     const float lp = job->l[j][row];
-                    job->w[j][row] = lp > 0.f ? ex2(job->w[j][row] - Mr[row]) : 0.f;
+                    job->w[j][row] = holds<VIS>(lp) ? ex2(job->w[j][row] - Mr[row]) : 0.f;
                 }
             __syncwarp();
             if (lane < ROWS) {
@@ -853,7 +863,7 @@ __device__ __forceinline__ void merge_warp_loop(const TiledParams& p, uint8_t* f
                 if (cb >= p.cta_start[c + 1]) continue;
                 const float* sl = p.slots + ((size_t)c * 2 + (max(a_flat, cb) != cb ? 1 : 0)) * kSlotFloats;
                 const float mp = __ldcg(sl + ROWS * D + lrow), lp = __ldcg(sl + ROWS * D + ROWS + lrow);
-                if (lp > 0.f) M = fmaxf(M, mp);
+                if (holds<VIS>(lp)) M = fmaxf(M, mp);
             }
 #pragma unroll 1
             for (int c = c_first; c <= c_last; ++c) {
@@ -861,7 +871,7 @@ __device__ __forceinline__ void merge_warp_loop(const TiledParams& p, uint8_t* f
                 if (cb >= p.cta_start[c + 1]) continue;
                 const float* sl = p.slots + ((size_t)c * 2 + (max(a_flat, cb) != cb ? 1 : 0)) * kSlotFloats;
                 const float mp = __ldcg(sl + ROWS * D + lrow), lp = __ldcg(sl + ROWS * D + ROWS + lrow);
-                const float wgt = lp > 0.f ? ex2(mp - M) : 0.f;
+                const float wgt = holds<VIS>(lp) ? ex2(mp - M) : 0.f;
                 den = fmaf(wgt, lp, den);
                 float v[ROWS][V];
                 load_rows(sl, v);
@@ -877,7 +887,7 @@ __device__ __forceinline__ void merge_warp_loop(const TiledParams& p, uint8_t* f
                 const long long dst = out_offset<D>(p, rq.qs + i, rq.head * p.G + hh) + V * lane;
                 float o[V];
 #pragma unroll
-                for (int k = 0; k < V; ++k) o[k] = dr > 0.f ? acc[row][k] / dr : 0.f;
+                for (int k = 0; k < V; ++k) o[k] = holds<VIS>(dr) ? acc[row][k] / dr : 0.f;
                 if constexpr (V == 4) {
                     uint2 packed;
                     packed.x = pack2<BF16>(o[0], o[1]);

@@ -368,6 +368,35 @@ __device__ __forceinline__ bool key_seen(const TiledParams& p, bool tree, int qs
     }
 }
 
+// Whether a row sum has something in it.  In the VIS builds a sum that is not a number counts, so that it reaches the output.
+template <bool VIS> __device__ __forceinline__ bool holds(float l) { return VIS ? l != 0.f : l > 0.f; }
+// A masked weight is an exact zero, but 0 * NaN is not: in a tile that some rows of a unit see and others do not, values of a
+// float pool that are not finite are replaced by zeros; the rows that see one get NaN for their sum instead.  Called by the
+// warp that reads the 16 value rows from `tok0` on; returns the rows (bit = token) in which there were any.
+template <int D, bool BF16>
+__device__ __forceinline__ uint32_t take_out_odd_values(uint8_t* v_tile, int tok0, int lane) {
+    constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+    uint32_t odd = 0;
+#pragma unroll 1
+    for (int c = lane; c < 16 * (D / 8); c += 32) {
+        const int tok = c / (D / 8), ch = c % (D / 8);
+        uint4* at = (uint4*)(v_tile + (ch >> 3) * (kTile * 128) + (tok0 + tok) * 128 + (ch & 7) * 16);
+        uint4 v = *at;
+        uint32_t* w = (uint32_t*)&v;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if ((w[e] & kExp) == kExp) { w[e] &= 0xffff0000u; bad = true; }
+            if (((w[e] >> 16) & kExp) == kExp) { w[e] &= 0x0000ffffu; bad = true; }
+        }
+        if (bad) { *at = v; odd |= 1u << tok; }
+    }
+    odd = __reduce_or_sync(0xffffffffu, odd);
+    if (odd) ptx::fence_proxy_async();  // the slot is refilled by TMA later
+    __syncwarp();
+    return odd;
+}
+
 // ------------------------------------------------------------------------------------------ producer
 template <int D, int NT, int FMT, bool VIS>
 __device__ __forceinline__ void producer_loop(const CUtensorMap* kmap, const CUtensorMap* vmap, const TiledParams& p,
@@ -853,6 +882,16 @@ __device__ __forceinline__ void consumer_loop(const TiledParams& p, uint8_t* sta
                         if (!key_seen<VIS>(p, tree, qs, i, ctx, kv_len, q_len, tok, row_lo[nt][c & 1], row_hi[nt][c & 1])) s[nt][c] = -INFINITY;
                     }
             }
+            if constexpr (VIS && FMT == 0) {
+                if (!interior && q_len > 1) {
+                    const uint32_t odd = take_out_odd_values<D, BF16>(st + C::KBYTES, 16 * warp, lane);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (((odd >> (c < 2 ? g : g + 8)) & 1) && s[nt][c] != -INFINITY) l[nt][c & 1] = __int_as_float(0x7fffffff);
+                }
+            }
             // tile maximum per row: own 16 tokens, then all warps through shared atomics
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -1075,7 +1114,7 @@ __device__ __forceinline__ void consumer_loop(const TiledParams& p, uint8_t* sta
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int e = c & 1, row = 8 * nt + 2 * t + e, d = 16 * ds + g + 8 * (c >> 1);
-                        const float inv = lsum[nt][e] > 0.f ? 1.0f / lsum[nt][e] : 0.f;
+                        const float inv = holds<VIS>(lsum[nt][e]) ? 1.0f / lsum[nt][e] : 0.f;
                         *(uint16_t*)(Ps + row * kPStride + d * 2) = to_bits16<BF16>(o[nt][c] * inv);
                     }
             }
@@ -1134,7 +1173,7 @@ __device__ __forceinline__ void consumer_loop(const TiledParams& p, uint8_t* sta
                         const long long cb = p.cta_start[c];
                         if (cb >= p.cta_start[c + 1]) continue;
                         const float* sl = p.slots + ((size_t)c * 2 + (max(a_flat, cb) != cb ? 1 : 0)) * kSlotFloats;
-                        if (__ldcg(sl + ROWS * D + ROWS + row) > 0.f) M = fmaxf(M, __ldcg(sl + ROWS * D + row));
+                        if (holds<VIS>(__ldcg(sl + ROWS * D + ROWS + row))) M = fmaxf(M, __ldcg(sl + ROWS * D + row));
                     }
                     float acc = 0.f, den = 0.f;
                     for (int c = c_first; c <= c_last; ++c) {
@@ -1142,14 +1181,14 @@ __device__ __forceinline__ void consumer_loop(const TiledParams& p, uint8_t* sta
                         if (cb >= p.cta_start[c + 1]) continue;
                         const float* sl = p.slots + ((size_t)c * 2 + (max(a_flat, cb) != cb ? 1 : 0)) * kSlotFloats;
                         const float lp = __ldcg(sl + ROWS * D + ROWS + row);
-                        if (lp > 0.f) {
+                        if (holds<VIS>(lp)) {
                             const float wgt = exp2f(__ldcg(sl + ROWS * D + row) - M);
                             acc += wgt * __ldcg(sl + row * D + d);
                             den += wgt * lp;
                         }
                     }
                     const int i = r / p.G, hh = r - i * p.G;
-                    store_out(p, out_offset<D>(p, qs + i, head * p.G + hh) + d, to_bits16<BF16>(den > 0.f ? acc / den : 0.f));
+                    store_out(p, out_offset<D>(p, qs + i, head * p.G + hh) + d, to_bits16<BF16>(holds<VIS>(den) ? acc / den : 0.f));
                 }
                 if (tid == 0) *counter = 0;  // ready for the next launch
                 if constexpr (PEER) {  // uniform over the consumer warps (the ticket is shared)
@@ -1245,7 +1284,7 @@ attn_tiled_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
 
     if (threadIdx.x >= kConsumerThreads + 32) {
         if constexpr (C::PRIVATE) {
-            merge_warp_loop<D, NT, FMT, BF16, PEER, HELP>(p, fixed, full, abort_word, (int)active);
+            merge_warp_loop<D, NT, FMT, BF16, PEER, HELP, VIS>(p, fixed, full, abort_word, (int)active);
             // no further job: consumer warps that are parked, or park later, may leave
             __syncwarp();
             if ((threadIdx.x & 31) == 0) {

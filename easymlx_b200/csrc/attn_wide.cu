@@ -76,9 +76,11 @@ struct WdBarriers {
     uint64_t item_full[4];
     uint64_t item_done;             // the item's rows are stored
     uint64_t xch;                   // exchange steps between the streams
+    uint64_t v_seen[4];             // per ring place: V has been looked over, and `odd` is that of its tile
     uint64_t turn[2];               // the tensor pipe is stream s's
     uint64_t drain;                 // every product of the CTA is complete
     int item_ring[4];
+    uint32_t odd[4][4];             // per ring place: tokens of the tile whose values are not all finite
     uint32_t tmem_base;
     int abort_word;
 };
@@ -155,6 +157,19 @@ __device__ __forceinline__ void drain_copies(uint64_t* bar) {
         ptx::mbar_wait(bar, parity, &never, 1u << 14);      // no copy: the wait runs out
     }
 }
+// Two 16-bit values: whether one of them is infinite or NaN (all exponent bits set), and the pair with zeros in place of such.
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint32_t v) {
+    constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+    return (v & kExp) == kExp || ((v >> 16) & kExp) == kExp;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite_only(uint32_t v) {
+    constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+    if ((v & kExp) == kExp) v &= 0xffff0000u;
+    if (((v >> 16) & kExp) == kExp) v &= 0x0000ffffu;
+    return v;
+}
 // The rare paths stay out of the tile loop's instruction stream: a warp runs through that loop's straight code once per
 // tile, and what lies between costs fetches even when it is skipped.
 //
@@ -220,6 +235,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             ptx::mbar_init(&bars->turn[s], 1);
         }
         for (int s = 0; s < 4; ++s) ptx::mbar_init(&bars->item_full[s], 1);
+        for (int s = 0; s < 4; ++s) ptx::mbar_init(&bars->v_seen[s], kRowBlock);
         ptx::mbar_init(&bars->item_done, kWdSoftThreads);
         ptx::mbar_init(&bars->xch, kWdSoftThreads);
         ptx::mbar_init(&bars->drain, 2);
@@ -454,6 +470,8 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             const int hi_min = tree ? ctx : min(kv_len, ctx + block0 / p.G + 1);
             const int lo_max = window_lo(p.vis, ctx, tree ? q_len : (block0 + rows_here - 1) / p.G + 1);
             const int lo_unit = unit_lo(p.vis, tree, row0, p.G, ctx, kv_len);
+            const int hi_unit = tree ? ctx : min(kv_len, ctx + row0 / p.G + 1);
+            const int lo_unit_max = window_lo(p.vis, ctx, tree ? q_len : (min(row0 + kWideRows, R) - 1) / p.G + 1);
             const int steps = pair ? it.count : (it.count - g + 1) / 2;
 
             float m_ref = -INFINITY, l = 0.f;
@@ -464,36 +482,68 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 ptx::mbar_wait(&bars->s_full[g], s_phase & 1, abort_word);
                 ++s_phase;
                 tc_fence_after();
-                // tokens of the tile that no row of the unit sees: their values are cleared (thread r owns token r).  The two
-                // streams of a pair share the tile; each clears it before its own product, and the second zero changes nothing
-                if (t0 + kTile > kv_len || (t0 < lo_unit && t0 + kTile > sinks)) {
-                    const uint32_t slot = 2 * (t % C::PLACES) + 1;
-                    ptx::mbar_wait(&bars->full[slot], uses.use_of(t) & 1, abort_word);
-                    const int tok = t0 + r;
-                    if (tok >= kv_len || (tok < lo_unit && tok >= sinks)) {
-#pragma unroll
-                        for (int h = 0; h < C::HALVES; ++h) {
-                            uint8_t* vrow = ring + (size_t)slot * C::TILE + h * (kTile * 128) + r * 128;
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) *(uint4*)(vrow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                    }
-                    ptx::fence_proxy_async();  // the tensor core reads V through the async proxy
-                }
-                if (!dead) {
-                    if (!whole) mask_scores(s_addr, [&](int b) {
-                        uint64_t seen = key_range(lo, hi, b) | key_range(0, min(sinks, hi), b);
-                        if (tree && b + 64 > ctx && b < kv_len) {
-                            const int j = b - ctx;  // new token that key b is
-                            if (j >= 0) {
-                                seen |= (j < 64 ? word0 : tree_word(p.vis, bits, j >> 6, q_len)) >> (j & 63);
-                                if ((j & 63) && p.vis.words > (j >> 6) + 1) seen |= tree_word(p.vis, bits, (j >> 6) + 1, q_len) << (64 - (j & 63));
-                            } else if (j > -64) {
-                                seen |= word0 << (-j);
+                // A masked weight is an exact zero, but 0 * NaN is not.  So in a tile that is not visible to the unit as a whole the
+                // values of tokens that no row sees are cleared, and so are values that are not finite at tokens that some
+                // rows may see and others not: the rows that do see one get NaN for their sum instead.  Thread r owns token r;
+                // where the streams share the tile, stream 0 does it for both.
+                const int place = t % C::PLACES;
+                const bool hidden = t0 + kTile > kv_len || (t0 < lo_unit && t0 + kTile > sinks);
+                const bool mixed = q_len > 1 && !(t0 + kTile <= hi_unit && (t0 >= lo_unit_max || t0 + kTile <= sinks));
+                uint64_t odd[2] = {0, 0};
+                if (!pair || g == 0) {
+                    if (hidden || mixed) {
+                        ptx::mbar_wait(&bars->full[2 * place + 1], uses.use_of(t) & 1, abort_word);
+                        const int tok = t0 + r;
+                        uint8_t* vrow = ring + (size_t)(2 * place + 1) * C::TILE + r * 128;
+                        const bool clear = tok >= kv_len || (tok < lo_unit && tok >= sinks);
+                        bool bad = false;
+                        if (mixed && !clear) {
+#pragma unroll 4
+                            for (int c = 0; c < 8 * C::HALVES; ++c) {
+                                const uint4 v = *(const uint4*)(vrow + (c >> 3) * (kTile * 128) + (c & 7) * 16);
+                                bad |= not_finite<BF16>(v.x) | not_finite<BF16>(v.y) | not_finite<BF16>(v.z) | not_finite<BF16>(v.w);
                             }
                         }
-                        return seen;
-                    }, t0);
+                        if (clear || bad) {
+#pragma unroll 1
+                            for (int c = 0; c < 8 * C::HALVES; ++c) {
+                                uint4* at = (uint4*)(vrow + (c >> 3) * (kTile * 128) + (c & 7) * 16);
+                                const uint4 v = *at;
+                                *at = clear ? make_uint4(0u, 0u, 0u, 0u)
+                                            : make_uint4(finite_only<BF16>(v.x), finite_only<BF16>(v.y), finite_only<BF16>(v.z), finite_only<BF16>(v.w));
+                            }
+                        }
+                        const uint32_t word = __ballot_sync(0xffffffffu, bad);
+                        if (lane == 0) bars->odd[place][warp & 3] = word;
+                        __syncwarp();
+                        ptx::fence_proxy_async();  // the tensor core reads V through the async proxy
+                    }
+                    ptx::mbar_arrive(&bars->v_seen[place]);
+                }
+                if (hidden || mixed) {
+                    ptx::mbar_wait(&bars->v_seen[place], uses.use_of(t) & 1, abort_word);
+                    odd[0] = pack2u(bars->odd[place][0], bars->odd[place][1]);
+                    odd[1] = pack2u(bars->odd[place][2], bars->odd[place][3]);
+                }
+                // the keys [b, b + 64) that this row sees
+                auto seen_at = [&](int b) {
+                    uint64_t seen = key_range(lo, hi, b) | key_range(0, min(sinks, hi), b);
+                    if (tree && b + 64 > ctx && b < kv_len) {
+                        const int j = b - ctx;  // new token that key b is
+                        if (j >= 0) {
+                            seen |= (j < 64 ? word0 : tree_word(p.vis, bits, j >> 6, q_len)) >> (j & 63);
+                            if ((j & 63) && p.vis.words > (j >> 6) + 1) seen |= tree_word(p.vis, bits, (j >> 6) + 1, q_len) << (64 - (j & 63));
+                        } else if (j > -64) {
+                            seen |= word0 << (-j);
+                        }
+                    }
+                    return seen;
+                };
+                if (odd[0] | odd[1]) {
+                    if ((seen_at(t0) & odd[0]) | (seen_at(t0 + 64) & odd[1])) l = __int_as_float(0x7fffffff);
+                }
+                if (!dead) {
+                    if (!whole) mask_scores(s_addr, seen_at, t0);
                     uint32_t sv[kTile];
 #pragma unroll
                     for (int c = 0; c < kTile / 32; ++c) tmem_ld32_nowait(s_addr + 32 * c, sv + 32 * c);
@@ -602,7 +652,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 if (!pair && g == 1) c_end = 0;  // stream 0 had the only tile
             }
             const bool store = block0 + r < R && !dead;
-            const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
+            const float inv = l_tot != 0.f ? 1.0f / l_tot : 0.f;  // (a sum that is not a number stays one)
             const int oi = (block0 + r) / p.G, ohh = (block0 + r) - oi * p.G;
             uint4* dst = (uint4*)((uint16_t*)p.out + ((long long)(qs + oi) * p.Hq + it.head * p.G + ohh) * D);
             float* slot = p.slots + (size_t)(it.slot) * C::SLOT_FLOATS;
@@ -701,7 +751,7 @@ __global__ void __launch_bounds__(256, 4) wide_combine_kernel(const __grid_const
         load(0);
         float M = -INFINITY;
         for (int j = lane; j < parts; j += 32)
-            if (__ldcg(base + j * kSlot + kWideRows * (D + 1) + sr) > 0.f) M = fmaxf(M, __ldcg(base + j * kSlot + kWideRows * D + sr));
+            if (__ldcg(base + j * kSlot + kWideRows * (D + 1) + sr) != 0.f) M = fmaxf(M, __ldcg(base + j * kSlot + kWideRows * D + sr));
         M = warp_max(M);
         float acc[V], den = 0.f;
 #pragma unroll
@@ -710,7 +760,7 @@ __global__ void __launch_bounds__(256, 4) wide_combine_kernel(const __grid_const
             const int jl = j0 + lane, n = min(32, parts - j0);
             const float lp = jl < parts ? __ldcg(base + jl * kSlot + kWideRows * (D + 1) + sr) : 0.f;
             const float mp = jl < parts ? __ldcg(base + jl * kSlot + kWideRows * D + sr) : -INFINITY;
-            const float w = lp > 0.f ? ex2(mp - M) : 0.f;
+            const float w = lp != 0.f ? ex2(mp - M) : 0.f;
             den += warp_sum(w * lp);
             for (int j = 0; j < n; j += kDeep) {
                 if (j0 + j > 0) load(j0 + j);
@@ -724,7 +774,7 @@ __global__ void __launch_bounds__(256, 4) wide_combine_kernel(const __grid_const
                 }
             }
         }
-        const float inv = den > 0.f ? 1.0f / den : 0.f;
+        const float inv = den != 0.f ? 1.0f / den : 0.f;
         const int oi = r / p.G, ohh = r - oi * p.G;
         uint32_t* dst = (uint32_t*)((uint16_t*)p.out + ((long long)(qs + oi) * p.Hq + head * p.G + ohh) * D + V * lane);
 #pragma unroll

@@ -88,6 +88,30 @@ def test_invisible_slots_may_hold_nan(bits, q, kernel):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("hq,hkv,d,dtype,n", [(8, 2, 128, FP16, 4), (8, 2, 64, BF16, 3), (6, 2, 128, FP16, 10), (8, 2, 128, BF16, 40), (16, 2, 64, FP16, 30),
+                                              (8, 8, 128, FP16, 12), (8, 2, 64, BF16, 100)])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(hq, hkv, d, dtype, n, kernel):
+    """A draft whose value row overflowed must not reach its siblings (nor a chunk's later token the earlier ones), while the
+    rows that see it do not come out finite."""
+    rng = np.random.default_rng(n)
+    for window, tree in ((0, True), (45, True), (45, False)):
+        b = Batch([150, 301, 20], [n] * 3, hq, hkv, d, 128, dtype, 0, seed=n, trees=[random_tree(rng, n) for _ in range(3)] if tree else None)
+        out, mass, reach = b.reference(d ** -0.5, window, 3)
+        hit = np.zeros(3 * n, bool)
+        for s in range(3):
+            ctx = b.ctx[s]
+            victims = [ctx + n // 2, ctx + n - 1, ctx - 10, 7]  # two drafts, a context key near the window's edge, one behind the sinks
+            for j, key in enumerate(victims):
+                b.arrays["value"][int(b.table[s, key // 128]), key % 128, j % hkv, (5 * j) % d] = [float("inf"), float("nan"), float("-inf"), float("nan")][j]
+            for i in range(n):
+                hit[s * n + i] = bool(set(b.line(s, i, window, 3)) & set(victims))
+        got = b.call(d ** -0.5, window, 3, kernel=kernel).double().cpu().numpy()
+        fine = np.abs(got - out) <= attention_bound(b, out, mass, reach)
+        assert fine[~hit].all()
+        assert (~np.isfinite(got)).reshape(3 * n, -1).any(-1)[hit].all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("page", [16, 128])
 def test_released_pages_between_sinks_and_window(page, kernel):
     """Pages that no row of the sequence sees any more may be gone from the table."""
