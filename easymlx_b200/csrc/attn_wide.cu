@@ -9,18 +9,24 @@
 // once for 256 rows; a smaller one deals its tiles to the streams alternately and joins the two states at the end.
 // Either way the tensor pipe works on one stream while the other stream's warps make exponentials: a 128 x 128 x 128
 // tile costs the tensor pipe 1024 cycles and the special-function unit (16 a clock) another 1024, and a single stream
-// would spend them one after the other.
+// would spend them one after the other.  What bounds it: a step of a stream takes 1700 cycles, 0.6 of the tensor pipe's rate,
+// of which S alone, with both operands from shared memory, is at what shared memory delivers.  Steps of 64 keys were 13 %
+// slower, streams that take no turns 15 %.  Measured: a prefill chunk of 2 x 2041 rows, 32 heads of 128, window 4096 and 16
+// sinks, 275 GFLOP, in 304 us with its work list (0.90 PFLOP/s); a step with 48 trees of 27 rows at contexts to 8192, where
+// the pool's bytes bound it, 886 MB in 184 us (4.8 TB/s).
 //
 // A row's running maximum is followed lazily: O in TMEM is rescaled only when the maximum has grown by more than 2^8, so
 // the stored weights stay below 2^15 and the row sum carries the same factor, which cancels in O / l.
+// Sums and states are 32-bit; weights are rounded to the pool's 16-bit type, as the tensor core takes its operands in one.
 //
 // Masks are 64-bit words: for a tile that is not visible as a whole, each thread forms the visibility of its row's 128
-// keys as two words (window, sinks, shifted tree mask) and tests constant bits.  Values at tokens that no row of the
-// unit sees are cleared in shared memory first, since 0 * NaN would reach the rows.
+// keys as two words (window, sinks, shifted tree mask) and tests constant bits.  A masked weight is zero, but 0 * NaN would
+// reach the rows: in tiles that some row sees in part only, one warp clears values that no row of the unit sees, and those
+// that are not finite; a row that sees one of these gets NaN.
 //
-// Warp roles: 0-3 stream 0, 4-7 stream 1, 8 TMA producer, 9 and 10 MMA issuers of the two
-// streams (9 owns the TMEM), 11 idle.  An issuing warp is held up until the tensor pipe has room for its instructions; with
-// a warp of its own, a stream's products are in the queue as soon as its weights are there.  All waits are bounded.
+// Warp roles: 0-3 stream 0, 4-7 stream 1, 8 TMA producer, 9 and 10 MMA issuers of the two streams (9 owns the TMEM), 11
+// looks values over.  An issuing warp is held up until the tensor pipe has room for its instructions; with a warp of its
+// own, a stream's products are in the queue as soon as its weights are there.  All waits are bounded.
 #include "tcgen05.cuh"
 #include "tensor_maps.cuh"
 #include "visible_plan.cuh"
@@ -29,7 +35,7 @@ namespace emlx {
 
 constexpr int kWdSoftThreads = 256;
 constexpr int kWdProducer = 8, kWdMma = 9;  // warps 9 and 10 issue the products of stream 0 and 1
-constexpr int kWdThreads = kWdSoftThreads + 128;  // whole warpgroups, since registers are moved between them (one warp idle)
+constexpr int kWdThreads = kWdSoftThreads + 128;  // whole warpgroups, since registers are moved between them
 // A softmax thread holds a row's 128 scores: it gets the registers that the copying and issuing warps do not need.
 // Together they stay inside what the block is launched with, 168 x 384.
 constexpr int kWdSoftRegs = 216, kWdOtherRegs = 72;
@@ -74,13 +80,13 @@ struct WdBarriers {
     uint64_t p_half[2], p_ready[2]; // per stream: P of the tile's first 64 keys written, all of P written
     uint64_t o_full[2];             // per stream: the item's last PV is complete
     uint64_t item_full[4];
-    uint64_t item_done;             // the item's rows are stored
+    uint64_t item_done[2];          // the rows of an item of this parity are stored
     uint64_t xch;                   // exchange steps between the streams
-    uint64_t v_seen[4];             // per ring place: V has been looked over, and `odd` is that of its tile
+    uint64_t v_seen[4];             // per ring place: its values have been looked over, and `odd` is that of its tile
     uint64_t turn[2];               // the tensor pipe is stream s's
     uint64_t drain;                 // every product of the CTA is complete
     int item_ring[4];
-    uint32_t odd[4][4];             // per ring place: tokens of the tile whose values are not all finite
+    alignas(16) uint32_t odd[4][4]; // per ring place: tokens of the tile whose values are not all finite
     uint32_t tmem_base;
     int abort_word;
 };
@@ -97,6 +103,28 @@ __device__ __forceinline__ WideItem wide_item(const WideParams& p, int idx) {
     it.slot += it.head * it.parts;
     return it;
 }
+// Which tiles hold values that some row of the unit must not meet: a masked weight is an exact zero, but 0 * NaN is not.
+// `clear(tok)`: no row of the unit sees the token.  `mixed`: some rows may see a token of the tile and others not.
+struct UnitValues {
+    int kv_len, sinks, lo, lo_max, hi;
+    bool rows;
+    __device__ __forceinline__ UnitValues(const WideParams& p, const WideItem& it) {
+        const int ctx = it.kv_len - it.q_len, R = it.q_len * p.G;
+        kv_len = it.kv_len;
+        sinks = p.vis.sinks;
+        rows = it.q_len > 1;
+        lo = unit_lo(p.vis, it.tree != 0, it.row0, p.G, ctx, kv_len);
+        lo_max = window_lo(p.vis, ctx, it.tree ? it.q_len : (min(it.row0 + kWideRows, R) - 1) / p.G + 1);
+        hi = it.tree ? ctx : min(kv_len, ctx + it.row0 / p.G + 1);
+    }
+    __device__ __forceinline__ bool clear(int tok) const { return tok >= kv_len || (tok < lo && tok >= sinks); }
+    __device__ __forceinline__ bool mixed(int t0) const {
+        return rows && ((t0 < lo_max && t0 + kTile > max(lo, sinks) && lo_max > sinks) || (t0 + kTile > hi && t0 < kv_len));
+    }
+    __device__ __forceinline__ bool touched(int t0) const {
+        return t0 + kTile > kv_len || (t0 < lo && t0 + kTile > sinks) || mixed(t0);
+    }
+};
 // Uses of the ring's places so far: every role counts them the same way, item by item.
 template <int PLACES>
 struct RingCount {
@@ -157,11 +185,12 @@ __device__ __forceinline__ void drain_copies(uint64_t* bar) {
         ptx::mbar_wait(bar, parity, &never, 1u << 14);      // no copy: the wait runs out
     }
 }
-// Two 16-bit values: whether one of them is infinite or NaN (all exponent bits set), and the pair with zeros in place of such.
+// Two 16-bit values: acc + 0 * v, which is NaN once a value is infinite or NaN, and the pair with zeros in place of such values.
 template <bool BF16>
-__device__ __forceinline__ bool not_finite(uint32_t v) {
-    constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-    return (v & kExp) == kExp || ((v >> 16) & kExp) == kExp;
+__device__ __forceinline__ uint32_t times_zero(uint32_t v, uint32_t acc) {
+    if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(acc) : "r"(v), "r"(0u), "r"(acc));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(acc) : "r"(v), "r"(0u), "r"(acc));
+    return acc;
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t finite_only(uint32_t v) {
@@ -235,8 +264,8 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             ptx::mbar_init(&bars->turn[s], 1);
         }
         for (int s = 0; s < 4; ++s) ptx::mbar_init(&bars->item_full[s], 1);
-        for (int s = 0; s < 4; ++s) ptx::mbar_init(&bars->v_seen[s], kRowBlock);
-        ptx::mbar_init(&bars->item_done, kWdSoftThreads);
+        for (int s = 0; s < 4; ++s) ptx::mbar_init(&bars->v_seen[s], 1);
+        for (int s = 0; s < 2; ++s) ptx::mbar_init(&bars->item_done[s], kWdSoftThreads);
         ptx::mbar_init(&bars->xch, kWdSoftThreads);
         ptx::mbar_init(&bars->drain, 2);
         bars->abort_word = 0;
@@ -281,11 +310,11 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 const int sinks_in = sink_tiles(p.vis.sinks, tile_lo);
                 const int lo = unit_lo(p.vis, it.tree != 0, row0, p.G, kv_len - q_len, kv_len);
                 // The item's Q replaces the last one's: every QK of that item must have read it, and where its streams joined
-                // their states through the same memory, its rows must be stored.  (The done phases are waited for in turn, so
-                // that none is two phases behind.)
+                // their states through the same memory, its rows must be stored.  (The done phases are waited for in turn, and
+                // alternate between two barriers, since the last item may be done as well: a wait two phases behind never ends.)
                 if (k > 0) {
                     const uint32_t need = last_pair ? k - 1 : k;
-                    for (; done_seen < need; ++done_seen) ptx::mbar_wait(&bars->item_done, done_seen & 1, abort_word);
+                    for (; done_seen < need; ++done_seen) ptx::mbar_wait(&bars->item_done[done_seen & 1], (done_seen >> 1) & 1, abort_word);
                     ptx::mbar_wait(&bars->q_free, (k - 1) & 1, abort_word);
                 }
                 last_pair = pair;
@@ -398,6 +427,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     const int t = pair ? i : 2 * i + s;
                     const uint32_t slot = 2 * (t % C::PLACES) + 1;
                     bool ok = ptx::mbar_wait(&bars->full[slot], uses.use_of(t) & 1, abort_word);
+                    ok = ptx::mbar_wait(&bars->v_seen[t % C::PLACES], uses.use_of(t) & 1, abort_word) && ok;
                     const uint64_t vd = v_desc0 + (uint64_t)(slot * (C::TILE >> 4));
                     // The product starts on the first 64 keys while the softmax warps are at the others.  The rest, and QK behind
                     // it, go in turn with the other stream: two streams that are in step would share the pipe and then the
@@ -432,6 +462,56 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             __syncwarp();
             int never = 0;  // (waited for even when another wait has given up)
             ptx::mbar_wait(&bars->drain, 0, &never);
+        } else {
+            // ------------------------------------------------------------------ values that are not for every row
+            // In a tile that some row sees in part only, the values of tokens that no row sees are cleared, and so are values
+            // that are not finite; the softmax threads are told where those were.  (One warp beside the tile loop: done by the
+            // softmax threads themselves it cost a prefill chunk 7 to 13 %, and so 1 %; four reads in flight, not eight: 4 % better.)
+            RingCount<C::PLACES> uses;
+            for (uint32_t k = 0;; ++k) {
+                if (!ptx::mbar_wait(&bars->item_full[k & 3], (k >> 2) & 1, abort_word)) break;
+                const int idx = bars->item_ring[k & 3];
+                if (idx < 0) break;
+                const WideItem it = wide_item(p, idx);
+                const int sinks_in = sink_tiles(p.vis.sinks, it.tile_lo);
+                const UnitValues values(p, it);
+                for (int t = 0; t < it.count; ++t) {
+                    const int place = t % C::PLACES, t0 = tile_of(it.j0 + t, sinks_in, it.tile_lo) * kTile;
+                    const bool mixed = values.mixed(t0);
+                    const bool loaded = ptx::mbar_wait(&bars->full[2 * place + 1], uses.use_of(t) & 1, abort_word);
+                    if (__all_sync(0xffffffffu, loaded) && values.touched(t0)) {
+#pragma unroll 1
+                        for (int w = 0; w < kTile / 32; ++w) {  // lane = token; eight neighbours start at different 16-byte pieces
+                            uint8_t* row = ring + (size_t)(2 * place + 1) * C::TILE + (32 * w + lane) * 128;
+                            const bool clear = values.clear(t0 + 32 * w + lane);
+                            uint32_t acc = 0;  // stays zero as long as every value times zero is
+                            if (mixed && !clear) {
+#pragma unroll 4
+                                for (int c = 0; c < 8 * C::HALVES; ++c) {
+                                    const uint4 v = *(const uint4*)(row + (c >> 3) * (kTile * 128) + ((c ^ lane) & 7) * 16);
+                                    acc = times_zero<BF16>(v.w, times_zero<BF16>(v.z, times_zero<BF16>(v.y, times_zero<BF16>(v.x, acc))));
+                                }
+                            }
+                            const bool bad = (acc & 0x7fff7fffu) != 0;
+                            const uint32_t word = __ballot_sync(0xffffffffu, bad);
+                            if (lane == 0) bars->odd[place][w] = word;
+                            if (clear || bad) {
+#pragma unroll 1
+                                for (int c = 0; c < 8 * C::HALVES; ++c) {
+                                    uint4* at = (uint4*)(row + (c >> 3) * (kTile * 128) + ((c ^ lane) & 7) * 16);
+                                    const uint4 v = *at;
+                                    *at = clear ? make_uint4(0u, 0u, 0u, 0u)
+                                                : make_uint4(finite_only<BF16>(v.x), finite_only<BF16>(v.y), finite_only<BF16>(v.z), finite_only<BF16>(v.w));
+                                }
+                            }
+                        }
+                        ptx::fence_proxy_async();  // the tensor core reads V through the async proxy
+                    }
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(&bars->v_seen[place]);
+                }
+                uses.finish(it.count);
+            }
         }
     } else {
         // ------------------------------------------------------------------ softmax: thread = row of stream g
@@ -469,9 +549,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             // bounds over the stream's rows, for tiles that need no mask
             const int hi_min = tree ? ctx : min(kv_len, ctx + block0 / p.G + 1);
             const int lo_max = window_lo(p.vis, ctx, tree ? q_len : (block0 + rows_here - 1) / p.G + 1);
-            const int lo_unit = unit_lo(p.vis, tree, row0, p.G, ctx, kv_len);
-            const int hi_unit = tree ? ctx : min(kv_len, ctx + row0 / p.G + 1);
-            const int lo_unit_max = window_lo(p.vis, ctx, tree ? q_len : (min(row0 + kWideRows, R) - 1) / p.G + 1);
+            const UnitValues values(p, it);
             const int steps = pair ? it.count : (it.count - g + 1) / 2;
 
             float m_ref = -INFINITY, l = 0.f;
@@ -482,49 +560,6 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                 ptx::mbar_wait(&bars->s_full[g], s_phase & 1, abort_word);
                 ++s_phase;
                 tc_fence_after();
-                // A masked weight is an exact zero, but 0 * NaN is not.  So in a tile that is not visible to the unit as a whole the
-                // values of tokens that no row sees are cleared, and so are values that are not finite at tokens that some
-                // rows may see and others not: the rows that do see one get NaN for their sum instead.  Thread r owns token r;
-                // where the streams share the tile, stream 0 does it for both.
-                const int place = t % C::PLACES;
-                const bool hidden = t0 + kTile > kv_len || (t0 < lo_unit && t0 + kTile > sinks);
-                const bool mixed = q_len > 1 && !(t0 + kTile <= hi_unit && (t0 >= lo_unit_max || t0 + kTile <= sinks));
-                uint64_t odd[2] = {0, 0};
-                if (!pair || g == 0) {
-                    if (hidden || mixed) {
-                        ptx::mbar_wait(&bars->full[2 * place + 1], uses.use_of(t) & 1, abort_word);
-                        const int tok = t0 + r;
-                        uint8_t* vrow = ring + (size_t)(2 * place + 1) * C::TILE + r * 128;
-                        const bool clear = tok >= kv_len || (tok < lo_unit && tok >= sinks);
-                        bool bad = false;
-                        if (mixed && !clear) {
-#pragma unroll 4
-                            for (int c = 0; c < 8 * C::HALVES; ++c) {
-                                const uint4 v = *(const uint4*)(vrow + (c >> 3) * (kTile * 128) + (c & 7) * 16);
-                                bad |= not_finite<BF16>(v.x) | not_finite<BF16>(v.y) | not_finite<BF16>(v.z) | not_finite<BF16>(v.w);
-                            }
-                        }
-                        if (clear || bad) {
-#pragma unroll 1
-                            for (int c = 0; c < 8 * C::HALVES; ++c) {
-                                uint4* at = (uint4*)(vrow + (c >> 3) * (kTile * 128) + (c & 7) * 16);
-                                const uint4 v = *at;
-                                *at = clear ? make_uint4(0u, 0u, 0u, 0u)
-                                            : make_uint4(finite_only<BF16>(v.x), finite_only<BF16>(v.y), finite_only<BF16>(v.z), finite_only<BF16>(v.w));
-                            }
-                        }
-                        const uint32_t word = __ballot_sync(0xffffffffu, bad);
-                        if (lane == 0) bars->odd[place][warp & 3] = word;
-                        __syncwarp();
-                        ptx::fence_proxy_async();  // the tensor core reads V through the async proxy
-                    }
-                    ptx::mbar_arrive(&bars->v_seen[place]);
-                }
-                if (hidden || mixed) {
-                    ptx::mbar_wait(&bars->v_seen[place], uses.use_of(t) & 1, abort_word);
-                    odd[0] = pack2u(bars->odd[place][0], bars->odd[place][1]);
-                    odd[1] = pack2u(bars->odd[place][2], bars->odd[place][3]);
-                }
                 // the keys [b, b + 64) that this row sees
                 auto seen_at = [&](int b) {
                     uint64_t seen = key_range(lo, hi, b) | key_range(0, min(sinks, hi), b);
@@ -539,22 +574,11 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     }
                     return seen;
                 };
-                if (odd[0] | odd[1]) {
-                    if ((seen_at(t0) & odd[0]) | (seen_at(t0 + 64) & odd[1])) l = __int_as_float(0x7fffffff);
-                }
                 if (!dead) {
                     if (!whole) mask_scores(s_addr, seen_at, t0);
                     uint32_t sv[kTile];
-#pragma unroll
-                    for (int c = 0; c < kTile / 32; ++c) tmem_ld32_nowait(s_addr + 32 * c, sv + 32 * c);
-                    tmem_wait_ld();
-                    // The first half's weights are made with the reference the row has, and the tile's maximum is taken beside
-                    // them, in issue slots the special-function unit leaves; only when it has outgrown the reference (the
-                    // first tile, rarely a later one) are they made again.
-                    // fp16 weights are stored as 2^(s - m_ref + 7): a key rounds to zero below 2^-32 of the reference only
-                    constexpr float kShift = BF16 ? 0.0f : 7.0f;
+                    uint64_t sum2[2] = {0, 0}, neg2 = 0;
                     const uint64_t scale2 = pack2f(p.scale_log2e, p.scale_log2e);
-                    uint64_t sum2[2], neg2;
                     auto weights = [&](int c) {  // 32 keys
                         uint32_t packed[16];
 #pragma unroll
@@ -569,6 +593,14 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                         }
                         tmem_st16_nowait(s_addr + 16 * c, packed);
                     };
+#pragma unroll
+                    for (int c = 0; c < kTile / 32; ++c) tmem_ld32_nowait(s_addr + 32 * c, sv + 32 * c);
+                    tmem_wait_ld();
+                    // The first half's weights are made with the reference the row has, and the tile's maximum is taken beside
+                    // them, in issue slots the special-function unit leaves; only when it has outgrown the reference (the
+                    // first tile, rarely a later one) are they made again.
+                    // fp16 weights are stored as 2^(s - m_ref + 7): a key rounds to zero below 2^-32 of the reference only
+                    constexpr float kShift = BF16 ? 0.0f : 7.0f;
 #pragma unroll 1
                     for (;;) {
                         const float neg_m = kShift - (m_ref == -INFINITY ? 0.f : m_ref);
@@ -605,6 +637,15 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     tmem_wait_st();
                 } else {
                     ptx::mbar_arrive(&bars->p_half[g]);
+                }
+                if (values.mixed(t0)) {  // a row that sees a value that is not finite gets NaN for its sum
+                    const int place = t % C::PLACES;
+                    ptx::mbar_wait(&bars->v_seen[place], uses.use_of(t) & 1, abort_word);
+                    const uint4 odd = *(const uint4*)bars->odd[place];
+                    if (odd.x | odd.y | odd.z | odd.w) {
+                        const uint64_t seen = (seen_at(t0) & pack2u(odd.x, odd.y)) | (seen_at(t0 + 64) & pack2u(odd.z, odd.w));
+                        if (seen) l = __int_as_float(0x7fffffff);
+                    }
                 }
                 tc_fence_before();
                 ptx::mbar_arrive(&bars->p_ready[g]);
@@ -699,7 +740,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
             o_phase[1] += other_ran ? 1 : 0;
             tc_fence_before();
             ptx::fence_proxy_async();  // the next item's Q arrives by TMA over the memory of the exchange
-            ptx::mbar_arrive(&bars->item_done);
+            ptx::mbar_arrive(&bars->item_done[k & 1]);
         }
     }
     tc_fence_before();

@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kDqThreads) dequant_pages_kernel(const Dequant
         }
         // values: codes [head][d][tok * BITS / 8] (tokens of one element contiguous); a thread takes four tokens of eight
         // elements, one load per element, and turns them round in registers (a byte load per code took 157 us for 16
-        // sequences of 4600 tokens, 8 heads of 128, where the bytes alone are worth 70; this way FIGURE)
+        // sequences of 4600 tokens, 8 heads of 128, where the bytes alone are worth 70; this way 133)
 #pragma unroll 2
         for (int it = tid; it < items / 4; it += kDqThreads) {
             const int tok = it % (bs / 4) * 4, ch = it / (bs / 4);

@@ -294,7 +294,9 @@ int emlx_attn_decode_gather(const emlx_attn_args* args, const emlx_pool* pool, v
  * A sequence has ctx = kv_len - q_len keys from earlier steps and q_len new ones.  The visible sequence of row i is the
  * context followed by the new keys whose mask bit is set, in slot order (causal: every new key up to itself); n_i is the
  * number of those.  A sliding window W keeps the entries of rank >= ctx + n_i - W, sink_tokens N the entries of rank < N
- * on top (without a window sinks mean nothing: all keys are visible).  A row that sees no key gets zeros. */
+ * on top (without a window sinks mean nothing: all keys are visible).  A row that sees no key gets zeros.
+ * Keys and values that a row does not see do not reach it, NaN and infinities included.  A row that does see a value that
+ * is not finite may get NaN in all of its elements. */
 typedef struct emlx_visibility {
     const uint64_t* tree_mask;  /* device [T, tree_words]: bit j % 64 of word j / 64 = the row sees new key j of its
                                  * sequence (itself only when its own bit is set); NULL = causal rows              */
