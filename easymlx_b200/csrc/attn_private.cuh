@@ -341,7 +341,7 @@ __device__ __forceinline__ void consumer_loop_private(const TiledParams& p, uint
                         __syncwarp();
                     }
                     if constexpr (VIS) {
-                        if (q_len > 1) {
+                        if (q_len > 1 || tree) {  // (a tree of one token may not see itself)
                             const uint32_t odd = take_out_odd_values<D, BF16>(st + C::KBYTES, 16 * warp, lane);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)

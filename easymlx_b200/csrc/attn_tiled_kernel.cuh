@@ -883,7 +883,7 @@ __device__ __forceinline__ void consumer_loop(const TiledParams& p, uint8_t* sta
                     }
             }
             if constexpr (VIS && FMT == 0) {
-                if (!interior && q_len > 1) {
+                if (!interior && (q_len > 1 || tree)) {
                     const uint32_t odd = take_out_odd_values<D, BF16>(st + C::KBYTES, 16 * warp, lane);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)

@@ -112,7 +112,7 @@ struct UnitValues {
         const int ctx = it.kv_len - it.q_len, R = it.q_len * p.G;
         kv_len = it.kv_len;
         sinks = p.vis.sinks;
-        rows = it.q_len > 1;
+        rows = it.q_len > 1 || it.tree != 0;  // (one token's rows agree, but a tree's bounds are not exact)
         lo = unit_lo(p.vis, it.tree != 0, it.row0, p.G, ctx, kv_len);
         lo_max = window_lo(p.vis, ctx, it.tree ? it.q_len : (min(it.row0 + kWideRows, R) - 1) / p.G + 1);
         hi = it.tree ? ctx : min(kv_len, ctx + it.row0 / p.G + 1);

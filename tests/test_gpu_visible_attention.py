@@ -112,6 +112,22 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(hq, hkv, d,
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (12, 1, 64), (32, 1, 128), (64, 1, 64)])
+@pytest.mark.parametrize("window", [0, 33])
+def test_a_single_draft_that_does_not_see_itself(hq, hkv, d, window, kernel):
+    """Trees of one token: a cleared bit hides the token's own row, whatever it holds, and widens the window by one."""
+    b = Batch([130, 128, 40, 0], [1] * 4, hq, hkv, d, 128, FP16, 0, seed=d, trees=[[-1]] * 4)
+    b.mask[:] = 0
+    b.mask[2] = 1
+    out, mass, reach = b.reference(d ** -0.5, window, 2)
+    for s in (0, 1, 3):
+        b.arrays["value"][int(b.table[s, b.ctx[s] // 128]), b.ctx[s] % 128] = float("nan")
+    got = b.call(d ** -0.5, window, 2, kernel=kernel).double().cpu().numpy()
+    assert (np.abs(got - out) <= attention_bound(b, out, mass, reach)).all()
+    assert (got[3] == 0).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("page", [16, 128])
 def test_released_pages_between_sinks_and_window(page, kernel):
     """Pages that no row of the sequence sees any more may be gone from the table."""
