@@ -407,6 +407,8 @@ class PageCacheView:
         memory is another one than last time."""
         kc, vc, bt, lens = self.key_cache, self.value_cache, self.block_tables, self.kv_lens
         at = (kc.data_ptr(), vc.data_ptr(), bt.data_ptr(), lens.data_ptr())
+        if self.is_affine:
+            at += (self.k_scales.data_ptr(), self.k_biases.data_ptr(), self.v_scales.data_ptr(), self.v_biases.data_ptr())
         row = self._commit
         if row is not None and row[3] == at and row[4] is kc and row[5] is vc and row[6] is bt and row[7] is lens:
             return row

@@ -149,15 +149,17 @@ __global__ void __launch_bounds__(kCommitThreads) commit_tree_kernel(const __gri
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    for (int y = 0; y < (int)gridDim.y; ++y) {
-        if (!p.layer[y].advance) continue;
-        for (int k = tid; k < p.S; k += kCommitThreads) {
-            // committed holds layer 0's result; a sequence that was left alone keeps its length
-            const int sl = p.slot_ids[k];
-            bool first = sl >= 0 && sl < p.num_slots;
-            for (int j = 0; j < k && first; ++j) first = p.slot_ids[j] != sl;
-            if (first) p.layer[y].kv_lens[sl] = __ldcg(p.committed + k);
-        }
+    for (int k = tid; k < p.S; k += kCommitThreads) {
+        // committed holds layer 0's result; a sequence that was left alone keeps its length, a slot named twice has the
+        // first one's
+        const int sl = p.slot_ids[k];
+        bool first = sl >= 0 && sl < p.num_slots;
+#pragma unroll 8
+        for (int j = 0; j < k; ++j) first = first && p.slot_ids[j] != sl;
+        if (!first) continue;
+        const int len = __ldcg(p.committed + k);
+        for (int y = 0; y < (int)gridDim.y; ++y)
+            if (p.layer[y].advance) p.layer[y].kv_lens[sl] = len;
     }
     if (tid == 0) *p.ticket = 0;
 }

@@ -29,13 +29,13 @@ class PagedAttentionInputs:
 def prepare_paged_attention_inputs(queries, keys, values, *, kv_cache: PageCacheView,
                                    query_start_loc: tp.Sequence[int] | PageMetadata,
                                    slot_ids: tp.Sequence[int] | None = None, rope: tp.Any = None,
-                                   sliding_window: int | None = None) -> PagedAttentionInputs:
+                                   sliding_window: int | None = None, advance: bool = True) -> PagedAttentionInputs:
     meta = query_start_loc if isinstance(query_start_loc, PageMetadata) else PageMetadata(
         query_start_loc=query_start_loc, sliding_window=int(sliding_window) if sliding_window is not None else 0)
     slots = slot_ids or getattr(meta, "slot_ids", None) or ()
     query_lens = (1,) * len(slots) if getattr(meta, "is_single_token_decode", False) and slots else None
     q, kc, vc, resolved = kv_cache.concatenate_to_cache(queries, keys, values, cache_metadata=meta, slot_ids=slots,
-                                                        query_lens=query_lens, rope=rope)
+                                                        query_lens=query_lens, rope=rope, advance=advance)
     return PagedAttentionInputs(queries=q, key_cache=kc, value_cache=vc, metadata=resolved)
 
 
@@ -47,10 +47,12 @@ class AttentionPerformer:
         self.executor = OperationExecutor.from_operations(mixin=OperationRegistry.create(attn_mechanism))
 
     def __call__(self, queries, keys, values, *, cache_view: PageCacheView, cache_metadata: PageMetadata | None,
-                 rope: tp.Any = None) -> torch.Tensor:
-        return self._forward_paged(queries, keys, values, cache_view=cache_view, cache_metadata=cache_metadata, rope=rope)
+                 rope: tp.Any = None, advance: bool = True) -> torch.Tensor:
+        """``advance=False`` leaves the stored lengths to a later ``commit_tree`` (a step whose rows are draft trees)."""
+        return self._forward_paged(queries, keys, values, cache_view=cache_view, cache_metadata=cache_metadata, rope=rope,
+                                   advance=advance)
 
-    def _forward_paged(self, queries, keys, values, *, cache_view, cache_metadata, rope) -> torch.Tensor:
+    def _forward_paged(self, queries, keys, values, *, cache_view, cache_metadata, rope, advance=True) -> torch.Tensor:
         batched = queries.ndim == 4
         if batched:
             b, l = queries.shape[0], queries.shape[1]
@@ -58,7 +60,7 @@ class AttentionPerformer:
             keys = keys.reshape(-1, keys.shape[-2], keys.shape[-1])
             values = values.reshape(-1, values.shape[-2], values.shape[-1])
         prepared = prepare_paged_attention_inputs(queries, keys, values, kv_cache=cache_view,
-                                                  query_start_loc=cache_metadata, rope=rope)
+                                                  query_start_loc=cache_metadata, rope=rope, advance=advance)
         if prepared.queries.shape[0] == 0:
             out = queries
         else:

@@ -215,3 +215,44 @@ def test_captured_step_and_commit():
     torch.cuda.synchronize()
     for step, e in zip(steps, expect):
         assert torch.equal(step.out, e)
+
+
+@pytest.mark.parametrize("bits", [None, 8, 4])
+def test_a_tree_and_a_causal_chunk_through_the_performer(bits):
+    """One step through the model's entry: a tree, a causal chunk and a finished slot; the tree keeps a path, the chunk all of
+    its tokens.  The cache is then that of a step with those tokens only, bit for bit."""
+    import easymlx_b200 as emlx
+
+    hq, hkv, d = 8, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    make = lambda n, h: torch.randn(n, h, d, generator=g, device="cuda").to(FP16)
+    caches = [emlx.PageCacheView.init(num_seqs=3, max_seq_len=256, num_kv_heads=hkv, head_dim=d, block_size=16,
+                                      cache_dtype=f"affine{bits}" if bits else None) for _ in range(2)]
+    for slot, ctx in ((2, 37), (0, 16)):
+        rows = (make(ctx, hkv), make(ctx, hkv))
+        for c in caches:
+            c.append(slot, *rows)
+    parents, chunk, path = [-1, 0, 0, 1, -1, 4], 21, [0, 2]
+    n = len(parents) + chunk
+    q, k, v = make(n, hq), make(n, hkv), make(n, hkv)
+    mask = torch.zeros(n, 1, dtype=torch.int64, device="cuda")
+    mask[: len(parents)] = emlx.build_tree_mask([parents], device="cuda")
+    meta = emlx.PageMetadata(query_start_loc=emlx.build_query_start_loc([len(parents), chunk]), slot_ids=(2, 0), tree_mask=mask,
+                             tree_seqs=torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+    performer = emlx.AttentionPerformer(scale=d ** -0.5)
+    out = performer(q, k, v, cache_view=caches[0], cache_metadata=meta, advance=False)
+    assert caches[0].kv_lens.tolist() == [16, 0, 37]
+    assert caches[0].commit_tree([2, 0], [path, list(range(chunk))]).tolist() == [39, 37]
+    assert caches[0].kv_lens.tolist() == [37, 0, 39]
+    keep = torch.tensor(path + list(range(len(parents), n)), device="cuda")
+    plain = emlx.PageMetadata(query_start_loc=emlx.build_query_start_loc([len(path), chunk]), slot_ids=(2, 0))
+    want = performer(q[keep], k[keep], v[keep], cache_view=caches[1], cache_metadata=plain)
+    # the same keys in other groupings: weights and outputs each rounded to fp16, |v| < 5.  Codes: keys may be rounded to fp16 on
+    # one side, a score moves by |q| |k| 2^-11 / 8 < 12 * 12 * 2^-14 and the output by twice that of |v|
+    bound = 4 * 5 * 2.0 ** -11 + (2 * 5 * 144 * 2.0 ** -14 if bits else 0)
+    assert (out[keep].float() - want.float()).abs().max() < bound
+    assert torch.equal(caches[0].kv_lens, caches[1].kv_lens)
+    for slot in (0, 2):
+        lens = [0, int(caches[0].kv_lens[slot])]
+        a, b = (c.gather_kv_cache(c.block_tables[slot:slot + 1], lens, out_dtype=torch.float32) for c in caches)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
