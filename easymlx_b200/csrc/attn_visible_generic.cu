@@ -2,7 +2,9 @@
 // fp32 queries and pools, affine pools.  Eight warps walk the visible keys of one (packed token, q head) row, every
 // eighth key each, with an fp32 online softmax, and their states are folded in warp order.  A key that a row does not
 // see is never read, so nothing that lies there (infinities, NaN, pages handed to another sequence) can reach the row.
-// Bound by the latency of one key after the other; the tiled kernels serve the geometries that matter.
+// Bound by the latency of one key after the other (one tree of 16 rows at 2045 keys, 32 heads of 128: 1.3 ms against 0.06 of
+// the tensor-core kernel, both with their host call; 8 trees of 16 at 2048 keys, heads of 256: 15.6 ms); the tiled kernels
+// serve the geometries that matter.
 #include "pool_view.cuh"
 #include "visible.cuh"
 

@@ -7,9 +7,10 @@
 //     O[128 rows x D] += P . V                tcgen05.mma, A from TMEM, V in place as an MN-major operand
 // A unit of more than 128 rows runs its two row blocks as the two streams over the same tiles, so a K/V tile is loaded
 // once for 256 rows; a smaller one deals its tiles to the streams alternately and joins the two states at the end.
-// Either way the tensor pipe works on one stream while the other stream's warps make exponentials: a 128 x 128 x 128
-// tile costs the tensor pipe 1024 cycles and the special-function unit (16 a clock) another 1024, and a single stream
-// would spend them one after the other.  What bounds it: a step of a stream takes 1700 cycles, 0.6 of the tensor pipe's rate,
+// Either way the tensor pipe works on one stream while the other stream's warps make exponentials: two 128 x 128 x 128
+// tiles, one per stream, cost the tensor pipe 1024 cycles and the special-function unit another 1024, and a single stream
+// would spend them one after the other.  What bounds it: the two steps take 1700 cycles, 0.6 of the tensor pipe's rate (46 %
+// of it and 50 % of the special-function unit's over a whole prefill chunk, masked and uneven tiles included),
 // of which S alone, with both operands from shared memory, is at what shared memory delivers.  Steps of 64 keys were 13 %
 // slower, streams that take no turns 15 %.  Measured: a prefill chunk of 2 x 2041 rows, 32 heads of 128, window 4096 and 16
 // sinks, 275 GFLOP, in 304 us with its work list (0.90 PFLOP/s); a step with 48 trees of 27 rows at contexts to 8192, where

